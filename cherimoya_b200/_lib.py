@@ -26,7 +26,7 @@ EXPORTED = (
     "chm_block_packed_bytes", "chm_pack_block", "chm_block_workspace_bytes",
     "chm_block_forward", "chm_forward_noalloc", "chm_noalloc_read_status", "chm_read_status",
     "chm_selftest_wait_timeout", "chm_last_launch_count", "chm_timing_enable",
-    "chm_timing_collect",
+    "chm_timing_collect", "chm_log_probs", "chm_log_probs_backward", "chm_distill",
 )
 TIMING_CLASSES = ("stem", "stats", "mlp", "profile_head", "count_head", "score", "other")
 
@@ -65,13 +65,33 @@ class Params(ctypes.Structure):
     ]
 
 
+class Rows(ctypes.Structure):
+    """chm_rows."""
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("n_groups", ctypes.c_int32),
+        ("n_examples", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("group_offset", ctypes.c_void_p),
+        ("group_size", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_row_stride", ctypes.c_int64),
+        ("mask_group_offset", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("grad_row_stride", ctypes.c_int64),
+        ("grad_group_offset", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+    ]
+
+
 _lib = None
 _load_error = None
 
 
 def _declare(lib):
     vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
-    desc_p = ctypes.POINTER(ModelDesc)
+    desc_p, rows_p = ctypes.POINTER(ModelDesc), ctypes.POINTER(Rows)
     sigs = {
         "chm_abi_version": (i32, []),
         "chm_error_string": (ctypes.c_char_p, [i32]),
@@ -95,6 +115,9 @@ def _declare(lib):
         "chm_read_status": (i32, [vp, vp]),
         "chm_noalloc_read_status": (i32, [vp]),
         "chm_selftest_wait_timeout": (i32, [vp, sz, vp]),
+        "chm_log_probs": (i32, [rows_p, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
+        "chm_log_probs_backward": (i32, [rows_p, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]),
+        "chm_distill": (i32, [rows_p, vp, vp, i32, i32, vp, ctypes.c_float, vp, i32, vp, vp, vp]),
         "chm_last_launch_count": (ctypes.c_int64, []),
         "chm_timing_enable": (None, [i32]),
         "chm_timing_collect": (i32, [ctypes.POINTER(ctypes.c_double),

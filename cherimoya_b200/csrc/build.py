@@ -14,8 +14,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libcherimoya_b200.so")
-SOURCES = [os.path.join(HERE, "chm_engine.cu")]
-DEPS = SOURCES + [os.path.join(HERE, f) for f in ("chm_kernels.cuh", "chm_ptx.cuh")] + [
+SOURCES = [os.path.join(HERE, f) for f in ("chm_engine.cu", "chm_likelihood.cu")]
+DEPS = SOURCES + [os.path.join(HERE, f) for f in (
+    "chm_kernels.cuh", "chm_likelihood.cuh", "chm_host.h", "chm_ptx.cuh")] + [
     os.path.join(ROOT, "include", "cherimoya_b200.h")]
 
 
@@ -35,7 +36,7 @@ def build(verbose=False, force=False):
     if not force and not needs_build():
         return LIB
     cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo",
-           "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-O2", "-o", LIB + ".tmp"] + SOURCES
+           "-std=c++17", "--threads", "0", "-shared", "-Xcompiler", "-fPIC,-O2", "-o", LIB + ".tmp"] + SOURCES
     if verbose:
         cmd[1:1] = ["-Xptxas", "-v"]
     res = subprocess.run(cmd, capture_output=True, text=True)

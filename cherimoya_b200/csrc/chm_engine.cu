@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/cherimoya_b200.h"
+#include "chm_host.h"
 #include "chm_kernels.cuh"
 
 using namespace chm;
@@ -178,6 +179,10 @@ void launch_k(bool pdl, void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem,
 }
 
 
+}  // namespace
+
+namespace chm {
+
 int launch_status() {
   ++g_launches;
   const cudaError_t e = cudaGetLastError();
@@ -187,6 +192,25 @@ int launch_status() {
   }
   return CHM_OK;
 }
+
+void launches_reset() { g_launches = 0; }
+
+ScopedLaunchTimer::ScopedLaunchTimer(int cls, cudaStream_t st) : cls_(cls), st_(st) {
+  if (!g_timing.enabled) return;
+  start_ = g_timing.get();
+  stop_ = g_timing.get();
+  cudaEventRecord(start_, st_);
+}
+
+ScopedLaunchTimer::~ScopedLaunchTimer() {
+  if (!start_) return;
+  cudaEventRecord(stop_, st_);
+  g_timing.pending.push_back({cls_, start_, stop_});
+}
+
+}  // namespace chm
+
+namespace {
 
 #define CHM_TRY(expr)              \
   do {                             \

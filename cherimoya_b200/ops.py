@@ -8,6 +8,7 @@ to another implementation. Fake (meta) implementations are registered so
 """
 
 import ctypes
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -399,3 +400,149 @@ def block_forward(x: torch.Tensor, packed: torch.Tensor, packed_offset: int, hid
 @block_forward.register_fake
 def _block_forward_fake(x, packed, packed_offset, hidden, dilation):
     return torch.empty_like(x)
+
+
+# ----------------------------------------------------------------- likelihood, distillation
+# Rows are given as (z, lead, n, stride, offsets, sizes): n examples `stride`
+# elements apart, group g's first entry at offsets[g] and sizes[g] entries long
+# (chm_rows); `lead` is the shape of the per-row results. The functions named
+# *_impl are the bodies of the custom ops of the same name: eager callers call
+# them directly and save the dispatcher's share of a small call.
+_LOGITS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@functools.lru_cache(maxsize=256)
+def _host_array(kind, values):
+    return (kind * len(values))(*values)
+
+
+def _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets, grad, grad_stride,
+                 grad_offsets, temperature):
+    keep = (_host_array(ctypes.c_int64, tuple(offsets)), _host_array(ctypes.c_int32, tuple(sizes)),
+            _host_array(ctypes.c_int64, tuple(mask_offsets)) if mask is not None else None,
+            _host_array(ctypes.c_int64, tuple(grad_offsets)) if grad is not None else None)
+    at = [ctypes.addressof(k) if k is not None else None for k in keep]
+    rows = _lib.Rows(z.data_ptr(), _LOGITS[z.dtype], len(sizes), n, stride, at[0], at[1],
+                     _addr(mask), mask_stride, at[2], _addr(grad), grad_stride, at[3], temperature)
+    rows.keep = keep               # the struct holds bare addresses
+    return rows
+
+
+def _on(device, fn, *args):
+    """fn(*args, stream) with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def log_probs_impl(z: torch.Tensor, mask: Optional[torch.Tensor], lead: List[int], n: int,
+                   stride: int, offsets: List[int], sizes: List[int], mask_stride: int,
+                   mask_offsets: List[int], targets: torch.Tensor, top_k: int, temperature: float,
+                   want_stats: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor,
+                                              torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Log probabilities of targets, entropy, log normaliser, top log
+    probabilities, top indices, and the statistics log_probs_backward reads."""
+    lib = _lib.load()
+    _require_cuda(z, "logits")
+    S, dev, lead = targets.shape[-1], z.device, tuple(lead)
+    lp = torch.empty(lead + (S,), dtype=torch.float32, device=dev)
+    h = torch.empty(lead, dtype=torch.float32, device=dev)
+    norm = torch.empty(lead, dtype=torch.float32, device=dev)
+    top = torch.empty(lead + (top_k,), dtype=torch.float32, device=dev)
+    at = torch.empty(lead + (top_k,), dtype=torch.int64, device=dev)
+    stats = torch.empty((n * len(sizes) if want_stats else 0, 2), dtype=torch.float32, device=dev)
+    rows = _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets, None, 0,
+                        (), temperature)
+    st = _on(dev, lib.chm_log_probs, rows, targets.data_ptr(), S, top_k, lp.data_ptr(),
+             h.data_ptr(), norm.data_ptr(), top.data_ptr(), at.data_ptr(),
+             stats.data_ptr() if want_stats else None)
+    _lib.check(st, "log_probs")
+    return lp, h, norm, top, at, stats
+
+
+log_probs = torch.library.custom_op("cherimoya_b200::log_probs", log_probs_impl, mutates_args=())
+
+
+@log_probs.register_fake
+def _log_probs_fake(z, mask, lead, n, stride, offsets, sizes, mask_stride, mask_offsets, targets,
+                    top_k, temperature, want_stats):
+    def f32(*shape):
+        return z.new_empty(shape, dtype=torch.float32)
+    return (f32(*lead, targets.shape[-1]), f32(*lead), f32(*lead), f32(*lead, top_k),
+            z.new_empty((*lead, top_k), dtype=torch.int64),
+            f32(n * len(sizes) if want_stats else 0, 2))
+
+
+def log_probs_backward_impl(z: torch.Tensor, mask: Optional[torch.Tensor], shape: List[int],
+                            n: int, stride: int, offsets: List[int], sizes: List[int],
+                            mask_stride: int, mask_offsets: List[int], grad_stride: int,
+                            grad_offsets: List[int], targets: torch.Tensor,
+                            top_indices: torch.Tensor, stats: torch.Tensor,
+                            entropy: torch.Tensor, g_log_probs: Optional[torch.Tensor],
+                            g_entropy: Optional[torch.Tensor], g_norm: Optional[torch.Tensor],
+                            g_top: Optional[torch.Tensor], temperature: float) -> torch.Tensor:
+    """Gradient of log_probs' outputs, a contiguous tensor of `shape`."""
+    lib = _lib.load()
+    _require_cuda(z, "logits")
+    grad = torch.empty(tuple(shape), dtype=z.dtype, device=z.device)
+    if grad.numel() == 0:
+        return grad
+    rows = _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets, grad,
+                        grad_stride, grad_offsets, temperature)
+    st = _on(z.device, lib.chm_log_probs_backward, rows, targets.data_ptr(), targets.shape[-1],
+             top_indices.data_ptr(), top_indices.shape[-1], stats.data_ptr(), entropy.data_ptr(),
+             _addr(g_log_probs), _addr(g_entropy), _addr(g_norm), _addr(g_top))
+    _lib.check(st, "log_probs_backward")
+    return grad
+
+
+log_probs_backward = torch.library.custom_op("cherimoya_b200::log_probs_backward",
+                                             log_probs_backward_impl, mutates_args=())
+
+
+@log_probs_backward.register_fake
+def _log_probs_backward_fake(z, mask, shape, *rest):
+    return z.new_empty(shape)
+
+
+def distill_impl(z: torch.Tensor, mask: Optional[torch.Tensor], shape: List[int], lead: List[int],
+                 n: int, stride: int, offsets: List[int], sizes: List[int], mask_stride: int,
+                 mask_offsets: List[int], grad_stride: int, grad_offsets: List[int],
+                 indices: torch.Tensor, log_probs: torch.Tensor, renormalize: bool,
+                 weight: Optional[torch.Tensor], scale: float, upstream: Optional[torch.Tensor],
+                 reduce: bool, want_grad: bool,
+                 temperature: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Distillation losses of the rows, their sum (with `reduce`), and the
+    gradient (with `want_grad`, a contiguous tensor of `shape`); what is not
+    wanted is empty."""
+    lib = _lib.load()
+    _require_cuda(z, "logits")
+    dev = z.device
+    losses = torch.empty(tuple(lead), dtype=torch.float32, device=dev)
+    loss = torch.empty(() if reduce else (0,), dtype=torch.float32, device=dev)
+    grad = torch.empty(tuple(shape) if want_grad else (0,), dtype=z.dtype, device=dev)
+    rows = _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets,
+                        grad if want_grad else None, grad_stride, grad_offsets, temperature)
+    st = _on(dev, lib.chm_distill, rows, indices.data_ptr(), log_probs.data_ptr(),
+             indices.shape[-1], renormalize, _addr(weight), scale, _addr(upstream),
+             1 if upstream is not None and upstream.dim() > 0 else 0, losses.data_ptr(),
+             loss.data_ptr() if reduce else None)
+    _lib.check(st, "distill")
+    return losses, loss, grad
+
+
+distill = torch.library.custom_op("cherimoya_b200::distill", distill_impl, mutates_args=())
+
+
+@distill.register_fake
+def _distill_fake(z, mask, shape, lead, n, stride, offsets, sizes, mask_stride, mask_offsets,
+                  grad_stride, grad_offsets, indices, log_probs, renormalize, weight, scale,
+                  upstream, reduce, want_grad, temperature):
+    return (z.new_empty(lead, dtype=torch.float32),
+            z.new_empty(() if reduce else (0,), dtype=torch.float32),
+            z.new_empty(shape if want_grad else (0,)))

@@ -97,3 +97,27 @@ class ExpectedCountsWrapper(torch.nn.Module):
             probs = torch.softmax(logits.reshape(n, -1), dim=-1).reshape(n, c, length)
             out.append(probs * y_counts[:, i, None, None])
         return torch.cat(out, dim=1)
+
+
+class TopCellsWrapper(torch.nn.Module):
+    """What a student is distilled from: per signal group the ``top_k`` most
+    likely cells of the joint softmax over the group's channels and positions
+    at ``temperature``, its entropy, and the log-counts. Returns
+    (top_log_probs (N, n_groups, top_k), top_indices (N, n_groups, top_k)
+    int64, entropy (N, n_groups), logcounts); run through ``predict`` it
+    reduces a data set's profiles to the lists ``distillation_loss`` takes. No
+    upstream counterpart."""
+
+    def __init__(self, model, top_k=32, temperature=1.0):
+        super().__init__()
+        self.model = model
+        self.top_k = top_k
+        self.temperature = temperature
+
+    def forward(self, X, X_ctl=None):
+        from .likelihood import profile_log_probs
+        y_logits, y_logcounts = self.model(X, X_ctl=X_ctl)
+        model = self.model.model if isinstance(self.model, ControlWrapper) else self.model
+        out = profile_log_probs(y_logits, top_k=self.top_k, signal_groups=model.signal_groups,
+                                temperature=self.temperature)
+        return out.top_log_probs, out.top_indices, out.entropy, y_logcounts

@@ -183,6 +183,86 @@ int32_t chm_variant(const chm_model_desc* desc, const void* packed, int32_t n_pa
                     float* d_logcount, float* jsd,
                     void* workspace, size_t workspace_bytes, chm_stream_t stream);
 
+/* ---- likelihood and distillation on profile logits ----
+ * No counterpart in the upstream project. A row is one categorical
+ * distribution: the flattened channels and positions of one signal group of
+ * one example. Row (n, g) has the index n * n_groups + g in every per-row
+ * array. Its entries are
+ *   z_v = logits[n * row_stride + group_offset[g] + v],  0 <= v < group_size[g]
+ * and take part when the mask (bytes, the same addressing with its own
+ * stride and offsets, non-zero = takes part) allows them and z_v > -inf; the
+ * others have probability 0 whatever they hold. Probabilities are the softmax
+ * of z / temperature over the entries that take part. A row with none has the
+ * normaliser -inf, the entropy 0, loss 0 and gradient 0; a row with NaN or
+ * +inf among them has no distribution and answers NaN.
+ * Neither call needs a workspace; every call can be captured in a graph. */
+typedef enum { CHM_LOGITS_F32 = 0, CHM_LOGITS_BF16 = 1, CHM_LOGITS_F16 = 2 } chm_logits_dtype;
+
+#define CHM_ROW_MAX_ENTRIES (1 << 20) /* entries of one row              */
+#define CHM_ROW_MAX_TARGETS 1024      /* given or listed entries per row */
+#define CHM_ROW_MAX_TOP 128           /* top entries per row             */
+
+typedef struct {
+    const void* logits;               /* device                                  */
+    int32_t dtype;                    /* chm_logits_dtype                        */
+    int32_t n_groups;
+    int64_t n_examples;
+    int64_t row_stride;               /* elements                                */
+    const int64_t* group_offset;      /* host, [n_groups], elements              */
+    const int32_t* group_size;        /* host, [n_groups], entries               */
+    const uint8_t* mask;              /* device, or NULL: every entry takes part */
+    int64_t mask_row_stride;          /* bytes                                   */
+    const int64_t* mask_group_offset; /* host, [n_groups], bytes                 */
+    void* grad;                       /* device, the logits' type, or NULL       */
+    int64_t grad_row_stride;          /* elements                                */
+    const int64_t* grad_group_offset; /* host, [n_groups], elements              */
+    float temperature;                /* in [1/1024, 1024]                       */
+} chm_rows;
+
+/* Per row: log probabilities of n_targets given entries (targets: int64,
+ * (rows, n_targets); a negative one is an empty place and gives 0, one past
+ * the row gives NaN, one that does not take part -inf), the entropy, the log
+ * normaliser, and the top_k most likely entries in descending order, equal
+ * logits by ascending index (places without an entry: -inf and index -1).
+ * Outputs fp32 (indices int64); each may be NULL when it is not wanted. stats
+ * (rows, 2) keeps the row's maximum and the log of its sum of
+ * exp((z - maximum) / T), which the backward call reads. */
+int32_t chm_log_probs(const chm_rows* rows, const int64_t* targets, int32_t n_targets,
+                      int32_t top_k, float* log_probs, float* entropy, float* log_normalizer,
+                      float* top_log_probs, int64_t* top_indices, float* stats,
+                      chm_stream_t stream);
+
+/* Gradient of chm_log_probs' outputs with respect to the logits, into
+ * rows->grad. stats and entropy are the forward's; each incoming gradient
+ * (fp32, the shape of its output) may be NULL for zero. A target without a
+ * finite log probability has no gradient. */
+int32_t chm_log_probs_backward(const chm_rows* rows, const int64_t* targets, int32_t n_targets,
+                               const int64_t* top_indices, int32_t top_k,
+                               const float* stats, const float* entropy,
+                               const float* g_log_probs, const float* g_entropy,
+                               const float* g_log_normalizer, const float* g_top_log_probs,
+                               chm_stream_t stream);
+
+/* Distillation from a teacher's listed entries: teacher_indices int64 and
+ * teacher_log_probs fp32, both (rows, n_listed). With P the teacher's and q
+ * the student's probabilities,
+ *   loss = T^2 (sum_u P_u log(P_u / q_u) + P_rest log(P_rest / q_rest)),
+ * the last term over the one outcome "none of the listed". P_u is
+ * exp(teacher_log_probs) and P_rest what is missing to 1; with renormalize
+ * non-zero, and where the listed mass exceeds 1 or no entry is left outside
+ * the list, P is scaled to sum to 1 over the list and P_rest is 0. Negative
+ * indices are empty places, entries that do not take part are dropped, an
+ * entry listed twice counts once with both masses, an index past the row
+ * makes the row's loss and gradient NaN. Row r is scaled by
+ *   weight[r] (NULL: 1) * scale * upstream[r * upstream_stride] (NULL: 1);
+ * a row of weight 0 is not looked at. Written where not NULL: row_loss
+ * (rows), and rows->grad, the gradient of the scaled losses' sum; with loss
+ * not NULL also their sum, which needs row_loss. */
+int32_t chm_distill(const chm_rows* rows, const int64_t* teacher_indices,
+                    const float* teacher_log_probs, int32_t n_listed, int32_t renormalize,
+                    const float* weight, float scale, const float* upstream,
+                    int32_t upstream_stride, float* row_loss, float* loss, chm_stream_t stream);
+
 /* ---- one Cheri Block (standalone CheriBlock.forward, upstream
  * cherimoya/cheri.py:1072-1082 -> _fwd_inf_forward, cheri.py:741-754) ---- */
 
