@@ -9,14 +9,19 @@ The library is plain CUDA C++ behind the C ABI of include/cherimoya_b200.h
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libcherimoya_b200.so")
-SOURCES = [os.path.join(HERE, f) for f in ("chm_engine.cu", "chm_likelihood.cu")]
+SOURCES = [os.path.join(HERE, f) for f in (
+    "chm_engine.cu", "chm_likelihood.cu", "chm_likelihood_f32.cu", "chm_likelihood_bf16.cu",
+    "chm_likelihood_f16.cu")]
 DEPS = SOURCES + [os.path.join(HERE, f) for f in (
-    "chm_kernels.cuh", "chm_likelihood.cuh", "chm_host.h", "chm_ptx.cuh")] + [
+    "chm_kernels.cuh", "chm_likelihood.cuh", "chm_likelihood_run.cuh", "chm_likelihood.h",
+    "chm_host.h", "chm_ptx.cuh")] + [
     os.path.join(ROOT, "include", "cherimoya_b200.h")]
 
 
@@ -35,18 +40,29 @@ def needs_build():
 def build(verbose=False, force=False):
     if not force and not needs_build():
         return LIB
-    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo",
-           "-std=c++17", "--threads", "0", "-shared", "-Xcompiler", "-fPIC,-O2", "-o", LIB + ".tmp"] + SOURCES
+    arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
+    flags = arch + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2"]
     if verbose:
-        cmd[1:1] = ["-Xptxas", "-v"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+        flags += ["-Xptxas", "-v"]
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SOURCES]
+        # one compiler per source, side by side
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            done = list(pool.map(lambda a: _nvcc(flags + ["-c", a[0], "-o", a[1]]),
+                                 zip(SOURCES, objs)))
+        log = "".join(done) + _nvcc(arch + ["-shared", "-o", LIB + ".tmp"] + objs)
+    if verbose:
+        sys.stderr.write(log)
+    os.replace(LIB + ".tmp", LIB)
+    return LIB
+
+
+def _nvcc(args):
+    res = subprocess.run([nvcc_path()] + args, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("nvcc failed building libcherimoya_b200.so")
-    if verbose:
-        sys.stderr.write(res.stderr)
-    os.replace(LIB + ".tmp", LIB)
-    return LIB
+    return res.stderr
 
 
 if __name__ == "__main__":

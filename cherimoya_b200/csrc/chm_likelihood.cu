@@ -7,7 +7,7 @@
 
 #include "../../include/cherimoya_b200.h"
 #include "chm_host.h"
-#include "chm_likelihood.cuh"
+#include "chm_likelihood.h"
 
 using namespace chm;
 
@@ -73,25 +73,16 @@ lk::Rows make_rows(const chm_rows* r, int g0, int ng) {
   return a;
 }
 
-// Runs launch(rows) for every run of up to kMaxGroups groups.
+// Runs launch(rows, their number) for every run of up to kMaxGroups groups.
 template <typename F>
 int each_launch(const chm_rows* r, F launch) {
   launches_reset();
   if (r->n_examples == 0) return CHM_OK;
   for (int g0 = 0; g0 < r->n_groups; g0 += lk::kMaxGroups) {
     const lk::Rows a = make_rows(r, g0, std::min(lk::kMaxGroups, r->n_groups - g0));
-    LK_TRY(launch(a));
+    LK_TRY(launch(a, r->n_examples * a.ng));
   }
   return CHM_OK;
-}
-
-template <typename F>
-int by_type(int dtype, F f) {
-  switch (dtype) {
-    case CHM_LOGITS_F32: return f(float());
-    case CHM_LOGITS_BF16: return f(__nv_bfloat16());
-    default: return f(__half());
-  }
 }
 
 }  // namespace
@@ -112,13 +103,12 @@ int32_t chm_log_probs(const chm_rows* rows, const int64_t* targets, int32_t n_ta
   const lk::ScoreArgs o{reinterpret_cast<const long long*>(targets), n_targets, top_k, log_probs,
                         entropy, log_normalizer, top_log_probs,
                         reinterpret_cast<long long*>(top_indices), stats};
-  return each_launch(rows, [&](const lk::Rows& a) {
-    const unsigned grid = (unsigned)(rows->n_examples * a.ng);
-    return by_type(rows->dtype, [&](auto t) {
-      ScopedLaunchTimer timer(kTimingScore, st);
-      lk::log_probs_kernel<decltype(t)><<<grid, 256, 0, st>>>(a, o);
-      return launch_status();
-    });
+  return each_launch(rows, [&](const lk::Rows& a, long long n) {
+    switch (rows->dtype) {
+      case CHM_LOGITS_F32: return lk::run_log_probs<float>(a, o, n, st);
+      case CHM_LOGITS_BF16: return lk::run_log_probs<__nv_bfloat16>(a, o, n, st);
+      default: return lk::run_log_probs<__half>(a, o, n, st);
+    }
   });
 }
 
@@ -140,13 +130,12 @@ int32_t chm_log_probs_backward(const chm_rows* rows, const int64_t* targets, int
                             reinterpret_cast<const long long*>(top_indices), n_targets, top_k,
                             stats, entropy, n_targets > 0 ? g_log_probs : nullptr,
                             g_entropy, g_log_normalizer, top_k > 0 ? g_top_log_probs : nullptr};
-  return each_launch(rows, [&](const lk::Rows& a) {
-    const unsigned grid = (unsigned)(rows->n_examples * a.ng);
-    return by_type(rows->dtype, [&](auto t) {
-      ScopedLaunchTimer timer(kTimingScore, st);
-      lk::log_probs_grad_kernel<decltype(t)><<<grid, 256, 0, st>>>(a, o);
-      return launch_status();
-    });
+  return each_launch(rows, [&](const lk::Rows& a, long long n) {
+    switch (rows->dtype) {
+      case CHM_LOGITS_F32: return lk::run_log_probs_grad<float>(a, o, n, st);
+      case CHM_LOGITS_BF16: return lk::run_log_probs_grad<__nv_bfloat16>(a, o, n, st);
+      default: return lk::run_log_probs_grad<__half>(a, o, n, st);
+    }
   });
 }
 
@@ -164,25 +153,14 @@ int32_t chm_distill(const chm_rows* rows, const int64_t* teacher_indices,
   const lk::DistillArgs o{reinterpret_cast<const long long*>(teacher_indices), teacher_log_probs,
                           n_listed, renormalize != 0, weight, upstream, scale, upstream_stride,
                           row_loss};
-  LK_TRY(each_launch(rows, [&](const lk::Rows& a) {
-    const unsigned grid = (unsigned)(rows->n_examples * a.ng);
-    const int largest = *std::max_element(a.size, a.size + a.ng);
-    const size_t smem = (size_t)((largest + 31) / 32) * 4;
-    return by_type(rows->dtype, [&](auto t) {
-      auto kernel = lk::distill_kernel<decltype(t)>;
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               CHM_ROW_MAX_ENTRIES / 8) != cudaSuccess)
-        return (int)CHM_ERR_CUDA;
-      ScopedLaunchTimer timer(kTimingScore, st);
-      kernel<<<grid, 256, smem, st>>>(a, o);
-      return launch_status();
-    });
+  LK_TRY(each_launch(rows, [&](const lk::Rows& a, long long n) {
+    switch (rows->dtype) {
+      case CHM_LOGITS_F32: return lk::run_distill<float>(a, o, n, st);
+      case CHM_LOGITS_BF16: return lk::run_distill<__nv_bfloat16>(a, o, n, st);
+      default: return lk::run_distill<__half>(a, o, n, st);
+    }
   }));
-  if (loss) {
-    ScopedLaunchTimer timer(kTimingScore, st);
-    lk::sum_rows_kernel<<<1, 1024, 0, st>>>(row_loss, rows->n_examples * rows->n_groups, loss);
-    LK_TRY(launch_status());
-  }
+  if (loss) LK_TRY(lk::run_sum_rows(row_loss, rows->n_examples * rows->n_groups, loss, st));
   return CHM_OK;
 }
 
