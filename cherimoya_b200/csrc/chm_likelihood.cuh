@@ -11,6 +11,7 @@
 #include <cstdint>
 
 #include "chm_likelihood.h"
+#include "chm_ptx.cuh"
 
 namespace chm {
 namespace lk {
@@ -126,87 +127,76 @@ template <typename T, int E = 0> __device__ __forceinline__ void drop_bits(uint4
   }
 }
 
-// One row of the launch. Its entries are seen as 16-byte vectors of the
-// aligned granules they lie in: entry v is element (v + ph) % N of vector
-// (v + ph) / N, so any start address reads and writes full vectors but for
-// the two at the ends, which go element by element and stay inside the row.
+// -inf over element e of a vector in shared memory order
+template <typename T>
+__device__ __forceinline__ uint4 neg_inf_vec() {
+  return make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
+}
+
+// Packed fp32 pairs (two lanes per instruction).
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<f2*>(&r);
+}
+
+// One row of the launch. Whatever address it starts at, its entries are
+// `head` single ones up to a 16-byte boundary, nin full vectors, and a few
+// single ones behind; no access leaves the row.
 template <typename T>
 struct Row {
   static constexpr int N = Vec<T>::N;
   const T* z;
   const uint8_t* mask;
   T* grad;
-  int size, ph, nvec;
+  int size, head, nin;
   long long index;
-  bool vec_store;                 // the gradient's rows lie in their granules alike
 
   __device__ __forceinline__ Row(const Rows& a, unsigned r) {
-    const unsigned n = r / (unsigned)a.ng, g = r - n * (unsigned)a.ng;
+    const unsigned n = a.ng == 1 ? r : r / (unsigned)a.ng, g = r - n * (unsigned)a.ng;
     z = static_cast<const T*>(a.z) + n * a.row_stride + a.off[g];
     mask = a.mask ? a.mask + n * a.mask_stride + a.moff[g] : nullptr;
     grad = a.grad ? static_cast<T*>(a.grad) + n * a.grad_stride + a.goff[g] : nullptr;
     size = a.size[g];
     index = (long long)n * a.n_groups + a.g0 + g;
-    ph = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-    nvec = size ? (size + ph + N - 1) / N : 0;
-    vec_store = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
+    const int ph = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+    head = min(size, (N - ph) & (N - 1));
+    nin = (size - head) / N;
+  }
+  // the gradient's row lies in its granules as the logits' row does
+  __device__ __forceinline__ bool vec_store() const {
+    return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
   }
   __device__ __forceinline__ float at(int v) const {
     return (mask && !mask[v]) ? neg_inf() : to_float(z[v]);
   }
-  // vector j; entries that do not take part, and places outside the row, are -inf
-  __device__ __forceinline__ uint4 load(int j) const {
-    const int v0 = j * N - ph;
-    uint4 r;
-    if (v0 >= 0 && v0 + N <= size) {
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                   : "l"(z + v0));
-    } else {
-      uint32_t w[4] = {Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf};
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int v = v0 + e;
-        if (v < 0 || v >= size) continue;
-        if constexpr (sizeof(T) == 4) {
-          w[e] = reinterpret_cast<const uint32_t*>(z)[v];
-        } else {
-          const uint32_t h = reinterpret_cast<const uint16_t*>(z)[v];
-          w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | (h << 16) : (w[e / 2] & 0xffff0000u) | h;
-        }
-      }
-      r = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    if (mask) drop_bits<T>(r, masked(v0));
-    return r;
-  }
-  // bits of the elements that the mask takes out
-  __device__ __forceinline__ uint32_t masked(int v0) const {
+  __device__ __forceinline__ const T* vec(int j) const { return z + head + (long long)j * N; }
+  // vector j with -inf over what the mask takes out
+  __device__ __forceinline__ void apply_mask(uint4& r, int j) const {
+    const uint8_t* m = mask + head + (long long)j * N;
     uint32_t b = 0;
-    if (v0 >= 0 && v0 + N <= size && (reinterpret_cast<uintptr_t>(mask + v0) & (N - 1)) == 0) {
+    if ((reinterpret_cast<uintptr_t>(m) & (N - 1)) == 0) {
 #pragma unroll
       for (int i = 0; i < N / 4; ++i) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(mask + v0)[i];
+        const uint32_t w = reinterpret_cast<const uint32_t*>(m)[i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) b |= ((w >> (8 * e)) & 0xffu) ? 0u : 1u << (4 * i + e);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int v = v0 + e;
-        if (v >= 0 && v < size && !mask[v]) b |= 1u << e;
-      }
+      for (int e = 0; e < N; ++e) b |= m[e] ? 0u : 1u << e;
     }
-    return b;
+    if (b) drop_bits<T>(r, b);
   }
-  __device__ __forceinline__ void store(int j, const float (&d)[N]) const {
-    const int v0 = j * N - ph;
-    if (vec_store && v0 >= 0 && v0 + N <= size) {
-      *reinterpret_cast<uint4*>(grad + v0) = Vec<T>::pack(d);
+  __device__ __forceinline__ void store(int j, const float (&d)[N], bool vec_store) const {
+    T* g = grad + head + (long long)j * N;
+    if (vec_store) {
+      *reinterpret_cast<uint4*>(g) = Vec<T>::pack(d);
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (v0 + e >= 0 && v0 + e < size) grad[v0 + e] = to_type<T>(d[e]);
+      for (int e = 0; e < N; ++e) g[e] = to_type<T>(d[e]);
     }
   }
 };
@@ -261,15 +251,58 @@ __device__ __forceinline__ void remote_store(uint32_t a, unsigned long long v) {
 
 constexpr int kMaxCluster = 8;
 
-// The vectors of one block of a row's cluster: [begin, end), in chunks of
-// kThreads * kVecs that a team holds in registers. Rows that fit one chunk
-// per block are read from memory once, whatever the passes over them.
-struct Share {
-  int begin, end;
-  __device__ __forceinline__ Share(int nvec, int rank, int blocks) {
-    const int per = (nvec + blocks - 1) / blocks;
-    begin = min(rank * per, nvec);
-    end = min(begin + per, nvec);
+// One block's part of a row: the vectors [begin, end), the entries [first,
+// last), and for the first threads of the row's two ends one single entry.
+template <typename T> struct Share {
+  int begin, end, first, last;
+  int edge;                        // this thread's single entry, or -1
+  __device__ __forceinline__ Share(const Row<T>& row, int rank, int blocks, int tid) {
+    constexpr int N = Vec<T>::N;
+    const int per = (row.nin + blocks - 1) / blocks;
+    begin = min(rank * per, row.nin);
+    end = min(begin + per, row.nin);
+    const int tail = row.head + row.nin * N;
+    first = rank == 0 ? 0 : row.head + begin * N;
+    last = rank == blocks - 1 ? row.size : row.head + end * N;
+    edge = -1;
+    if (rank == 0 && tid < row.head) edge = tid;
+    else if (rank == blocks - 1 && tid >= N && tail + tid - N < row.size) edge = tail + tid - N;
+  }
+};
+
+// The vectors of a chunk pass through shared memory by asynchronous copies:
+// thread t copies, and alone reads, the vectors t, t + kThreads, ... of the
+// chunk, so it needs no barrier, all copies are in flight at once without a
+// register, and a row that fits is there for every later pass. Four groups,
+// so that the sums begin while most of the chunk is on its way.
+template <typename T, int kThreads>
+struct Stage {
+  uint4* buf;                      // this thread's first slot
+  int per;                         // vectors per group and thread
+  __device__ __forceinline__ Stage(uint4* chunk, int cap)
+      : buf(chunk + Team<kThreads>::tid()), per((cap / kThreads + 3) / 4) {}
+  // vectors of [base, end) that this thread has
+  __device__ __forceinline__ int count(int base, int end) const {
+    return max(0, end - base - Team<kThreads>::tid() + kThreads - 1) / kThreads;
+  }
+  __device__ __forceinline__ void copy(const Row<T>& row, int base, int n) const {
+    const T* src = row.vec(base + Team<kThreads>::tid());
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      const int e = min(n, (q + 1) * per);
+#pragma unroll 4
+      for (int i = q * per; i < e; ++i)
+        cp_async16(buf + i * kThreads, src + (long long)i * kThreads * Vec<T>::N, true);
+      cp_async_commit();
+    }
+  }
+  __device__ __forceinline__ void wait(int q) const {
+    switch (q) {
+      case 0: cp_async_wait<3>(); break;
+      case 1: cp_async_wait<2>(); break;
+      case 2: cp_async_wait<1>(); break;
+      default: cp_async_wait<0>();
+    }
   }
 };
 
@@ -285,12 +318,20 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c) {
   const float fa = ex2(da), fb = ex2(db);
   return {m, fa * a.s + fb * b.s, fa * (a.t + da * a.s) + fb * (b.t + db * b.s)};
 }
-// Adds a vector set of known maximum to the running sums.
+__device__ __forceinline__ Sums single(float z, float c) {
+  if (z == neg_inf()) return {z, 0.f, 0.f};
+  return {z, ex2((z - z) * c), 0.f};              // NaN for NaN and +inf
+}
+// Adds vectors to the running sums: per entry one exponential, half an add, a
+// product and two sums each, and a clamp for the entropy's 0 * -inf.
 template <typename T, int kVecs, bool kEntropy>
-__device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float top, float c, Sums& a) {
+__device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float c, Sums& a) {
   constexpr int N = Vec<T>::N;
-  if (top > a.m) {                            // a.m = -inf: nothing to rescale yet
-    if (a.m != neg_inf()) {
+  float top = Vec<T>::max(r[0]);
+#pragma unroll
+  for (int i = 1; i < kVecs; ++i) top = fmaxf(top, Vec<T>::max(r[i]));
+  if (top > a.m) {
+    if (a.m != neg_inf()) {                       // else nothing to rescale yet
       const float d = fmaxf((a.m - top) * c, -1000.f), f = ex2(d);
       if (kEntropy) a.t = f * (a.t + d * a.s);
       a.s *= f;
@@ -298,27 +339,33 @@ __device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float top, f
     a.m = top;
   }
   const float ref = a.m == neg_inf() ? 0.f : a.m;
-  float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+  const f2 nref = {-ref, -ref}, cc = {c, c};
+  f2 s = {0.f, 0.f}, t = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     float f[N];
     Vec<T>::unpack(r[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = (f[e] - ref) * c, p = ex2(x);
-      s[e & 1] += p;
-      if (kEntropy) t[e & 1] = fmaf(p, fmaxf(x, -1000.f), t[e & 1]);
+    for (int e = 0; e < N; e += 2) {
+      f2 x = mul2(add2(f2{f[e], f[e + 1]}, nref), cc);
+      const f2 p = {ex2(x.x), ex2(x.y)};
+      s = add2(s, p);
+      if (kEntropy) {
+        x.x = fmaxf(x.x, -1000.f);
+        x.y = fmaxf(x.y, -1000.f);
+        t = fma2(p, x, t);
+      }
     }
   }
-  a.s += s[0] + s[1];
-  if (kEntropy) a.t += t[0] + t[1];
+  a.s += s.x + s.y;
+  if (kEntropy) a.t += t.x + t.y;
 }
 
 // Joins the team's sums (every thread gets the result).
 template <int kThreads>
 __device__ __forceinline__ Sums team_sums(Sums a, float c, Sums* red) {
   using Tm = Team<kThreads>;
-#pragma unroll
+#pragma unroll 1
   for (int o = 16; o > 0; o >>= 1) {
     const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
                  __shfl_xor_sync(0xffffffffu, a.t, o)};
@@ -328,7 +375,7 @@ __device__ __forceinline__ Sums team_sums(Sums a, float c, Sums* red) {
   if (Tm::lane() == 0) red[Tm::warp()] = a;
   __syncthreads();
   a = red[0];
-#pragma unroll
+#pragma unroll 1
   for (int w = 1; w < Tm::kWarps; ++w) a = join(a, red[w], c);
   return a;
 }
@@ -373,52 +420,90 @@ template <int kThreads> struct TopShared {
   int red[Team<kThreads>::kWarps];
 };
 
-// Calls f(z, v) for every entry of the chunk that this thread holds.
-template <typename T, int kThreads, int kVecs, typename F>
-__device__ __forceinline__ void each_entry(const Row<T>& row, const uint4 (&r)[kVecs], int base,
-                                           int end, F f) {
+// Calls f(z, v) for this thread's entries of the share with z >= least (all,
+// where that is -inf), copying the chunks again if there are several.
+template <typename T, int kThreads, bool kMask, typename F>
+__device__ __forceinline__ void each_entry(const Row<T>& row, const Share<T>& share,
+                                           const Stage<T, kThreads>& st, int cap, float edge,
+                                           float least, F f) {
   constexpr int N = Vec<T>::N;
+  if (share.edge >= 0 && edge >= least) f(edge, share.edge);
+#pragma unroll 1
+  for (int base = share.begin; base < share.end; base += cap) {
+    const int n = st.count(base, min(base + cap, share.end));
+    if (share.end - share.begin > cap) {
+      st.copy(row, base, n);
+      cp_async_wait<0>();
+    }
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int j = base + i * kThreads + Team<kThreads>::tid();
+      uint4 r = st.buf[i * kThreads];
+      if (kMask && share.end - share.begin > cap) row.apply_mask(r, j);
+      if (!(Vec<T>::max(r) >= least)) continue;
+      float z[N];
+      Vec<T>::unpack(r, z);
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int j = base + i * kThreads + Team<kThreads>::tid();
-    if (j >= end) continue;
-    float z[N];
-    Vec<T>::unpack(r[i], z);
-#pragma unroll
-    for (int e = 0; e < N; ++e) f(z[e], j * N - row.ph + e);
+      for (int e = 0; e < N; ++e)
+        if (z[e] >= least) f(z[e], row.head + j * N + e);
+    }
   }
 }
 
-template <typename T, int kThreads, int kVecs>
-__device__ __forceinline__ void load_chunk(const Row<T>& row, const Share& sh, int base,
-                                           uint4 (&r)[kVecs]) {
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int j = base + i * kThreads + Team<kThreads>::tid();
-    if (j < sh.end) r[i] = row.load(j);
-    else r[i] = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
-  }
-}
-
-// The share's k largest entries, in no order, into sh.cand; returns their
-// number (at least k of them are there unless the share has fewer).
-//
-// Each thread has the maximum of its entries. With the maxima of a warp
-// sorted, min over the warps of the ceil(k / warps)-th is a value that at
-// least k entries reach, and so is the k-th of any one warp; every entry at
-// or above the larger of the two is a candidate. On entries in no order that
-// leaves about 2k of them (measured 1.1k to 2.5k). Rows that defeat the bound
-// (many equal logits, sorted rows) are counted instead: bisection for the
-// k-th largest logit, then for the index up to which its equals belong.
-template <typename T, int kThreads, int kVecs>
-__device__ int collect_top(const Row<T>& row, const Share& share, uint4 (&r)[kVecs], float top,
-                           int k, TopShared<kThreads>& sh) {
+// Rows that defeat the bound of collect_top (many equal logits, sorted rows)
+// are counted: bisection for the k-th largest logit, then for the index up to
+// which its equals belong to the first k. Leaves exactly k candidates.
+template <typename T, int kThreads, bool kMask>
+__device__ __noinline__ int count_top(const Row<T>& row, const Share<T>& share,
+                                      const Stage<T, kThreads>& st, int cap, float edge,
+                                      uint32_t bound, int k, TopShared<kThreads>& sh) {
   using Tm = Team<kThreads>;
-  constexpr int kChunk = kThreads * kVecs;
-  const bool one = share.end - share.begin <= kChunk;
+  // how many entries have a key of at least q (with `equal`: of exactly q, up to index v)
+  auto count = [&](uint32_t q, bool equal, int last) {
+    int n = 0;
+    each_entry<T, kThreads, kMask>(row, share, st, cap, edge, neg_inf(), [&](float z, int v) {
+      const uint32_t key = logit_key(z);
+      n += equal ? key == q && v <= last : key >= q;
+    });
+    return Tm::sum(n, sh.red);
+  };
+  uint32_t lo = max(bound, 1u), hi = 0xffffffffu;      // count(lo) >= k > count(hi)
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (count(mid, false, 0) >= k) lo = mid; else hi = mid;
+  }
+  const int need = k - count(hi, false, 0);
+  int before = -1, last = row.size - 1;                // equals up to `last`: at least `need`
+  while (last - before > 1) {
+    const int mid = before + (last - before) / 2;
+    if (count(lo, true, mid) >= need) last = mid; else before = mid;
+  }
+  Tm::sync();
   if (Tm::tid() == 0) sh.count = 0;
-  const uint32_t mine = warp_sort(logit_key(top));
-  sh.sorted[Tm::warp()][Tm::lane()] = mine;
+  Tm::sync();
+  each_entry<T, kThreads, kMask>(row, share, st, cap, edge, neg_inf(), [&](float z, int v) {
+    const uint32_t key = logit_key(z);
+    if (key > lo || (key == lo && v <= last)) sh.cand[atomicAdd(&sh.count, 1)] = order_key(key, v);
+  });
+  Tm::sync();
+  return sh.count;
+}
+
+// The k largest entries of a block's share and some more, in no order, into
+// sh.cand; returns their number (all there are if the share has fewer than k).
+//
+// Each thread knows the maximum of its entries. With the maxima of a warp
+// sorted, at least k entries reach the smallest over the warps of the
+// ceil(k / warps)-th, and k reach the k-th of any one warp; every entry at or
+// above the larger of the two is a candidate, on entries in no order about 2k
+// of them. Only threads whose maximum reaches the bound look again.
+template <typename T, int kThreads, bool kMask>
+__device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& share,
+                                           const Stage<T, kThreads>& st, int cap, float edge,
+                                           float top, int k, TopShared<kThreads>& sh) {
+  using Tm = Team<kThreads>;
+  if (Tm::tid() == 0) sh.count = 0;
+  sh.sorted[Tm::warp()][Tm::lane()] = warp_sort(logit_key(top));
   Tm::sync();
   const int each = (k + Tm::kWarps - 1) / Tm::kWarps;
   uint32_t low = 0xffffffffu, high = 0u;
@@ -428,61 +513,23 @@ __device__ int collect_top(const Row<T>& row, const Share& share, uint4 (&r)[kVe
     high = max(high, k <= 32 ? sh.sorted[w][k - 1] : 0u);
   }
   const uint32_t bound = max(low, high);
-  const float least = bound ? key_logit(bound) : neg_inf();
-  for (int base = share.begin; base < share.end; base += kChunk) {
-    if (!one) load_chunk<T, kThreads, kVecs>(row, share, base, r);
-    if (one && top < least) continue;
-    each_entry<T, kThreads>(row, r, base, share.end, [&](float z, int v) {
-      if (z >= least && z > neg_inf()) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kMaxCand) sh.cand[at] = order_key(logit_key(z), v);
-      }
+  const float least = bound ? key_logit(bound) : -3.4028234664e38f;   // the lowest logit there is
+  if (!(top < least))
+    each_entry<T, kThreads, kMask>(row, share, st, cap, edge, least, [&](float z, int v) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kMaxCand) sh.cand[at] = order_key(logit_key(z), v);
     });
-  }
   Tm::sync();
-  if (sh.count <= kMaxCand) return sh.count;
-
-  // how many entries have a key of at least q (of exactly q up to index v, with `equal`)
-  auto count = [&](uint32_t q, bool equal, int last) {
-    int n = 0;
-    for (int base = share.begin; base < share.end; base += kChunk) {
-      if (!one) load_chunk<T, kThreads, kVecs>(row, share, base, r);
-      each_entry<T, kThreads>(row, r, base, share.end, [&](float z, int v) {
-        const uint32_t key = logit_key(z);
-        n += equal ? key == q && v <= last : key >= q;
-      });
-    }
-    return Tm::sum(n, sh.red);
-  };
-  uint32_t lo = max(bound, 1u), hi = 0xffffffffu;      // count(lo) >= k > count(hi)
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (count(mid, false, 0) >= k) lo = mid; else hi = mid;
-  }
-  const int need = k - count(hi, false, 0);
-  int first = -1, last = row.size - 1;                 // equals up to `last`: at least `need`
-  while (last - first > 1) {
-    const int mid = first + (last - first) / 2;
-    if (count(lo, true, mid) >= need) last = mid; else first = mid;
-  }
-  Tm::sync();
-  if (Tm::tid() == 0) sh.count = 0;
-  Tm::sync();
-  for (int base = share.begin; base < share.end; base += kChunk) {
-    if (!one) load_chunk<T, kThreads, kVecs>(row, share, base, r);
-    each_entry<T, kThreads>(row, r, base, share.end, [&](float z, int v) {
-      const uint32_t key = logit_key(z);
-      if (key > lo || (key == lo && v <= last)) sh.cand[atomicAdd(&sh.count, 1)] = order_key(key, v);
-    });
-  }
-  Tm::sync();
-  return sh.count;
+  const int n = sh.count;
+  if (n <= kMaxCand) return n;
+  return count_top<T, kThreads, kMask>(row, share, st, cap, edge, bound, k, sh);
 }
 
 // Place of a key among `n` different ones, the largest first.
 __device__ __forceinline__ int rank_of(unsigned long long key, const unsigned long long* keys,
                                        int n) {
   int r = 0;
+#pragma unroll 4
   for (int i = 0; i < n; ++i) r += keys[i] > key;
   return r;
 }
@@ -493,41 +540,64 @@ template <int kThreads> struct ScoreShared {
   TopShared<kThreads> top;
 };
 // What the other blocks of a row's cluster send to the first.
-template <int kBlocks> struct ScoreCluster {
-  float sums[kBlocks][4];
-  unsigned long long keys[kBlocks][kMaxTop];
+struct ScoreCluster {
+  float sums[kMaxCluster][4];
+  unsigned long long keys[kMaxCluster][kMaxTop];
 };
 
-// One pass over the row for maximum, sum and entropy, the top entries from
-// the registers, and the given entries by a gather at the end.
-template <typename T, int kThreads, int kVecs, int kMinBlocks>
-__global__ void __launch_bounds__(Team<kThreads>::kBlock, kMinBlocks)
-log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned rows, int blocks) {
+// One pass over the row for maximum, sum and entropy; the top entries from
+// the row in shared memory; the given entries by a gather at the end.
+// Dynamic shared memory: per team `cap` vectors; ScoreCluster if blocks > 1.
+template <typename T, int kThreads, bool kMask>
+__global__ void __launch_bounds__(Team<kThreads>::kBlock)
+log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned rows, int blocks,
+                 int cap) {
   using Tm = Team<kThreads>;
-  constexpr int kChunk = kThreads * kVecs;
+  extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ ScoreShared<kThreads> shared[Tm::kPerBlock];
-  __shared__ ScoreCluster<kThreads >= 256 ? kMaxCluster : 1> cl;
   ScoreShared<kThreads>& sh = shared[Tm::slot()];
+  uint4* chunk = reinterpret_cast<uint4*>(dyn) + Tm::slot() * cap;
+  ScoreCluster& cl = *reinterpret_cast<ScoreCluster*>(dyn + cap * 16);
   const unsigned r0 = blockIdx.x / blocks * Tm::kPerBlock + Tm::slot();
   const int rank = blockIdx.x % blocks;
   if (kThreads == 32 && r0 >= rows) return;            // a whole warp, and no cluster
   if (blocks > 1) cluster_arrive();                    // the blocks of the cluster have begun
   const Row<T> row(a, r0);
-  const Share share(row.nvec, rank, blocks);
-  uint4 r[kVecs];
+  const Share<T> share(row, rank, blocks, Tm::tid());
+  const Stage<T, kThreads> st(chunk, cap);
+  float edge = neg_inf();
+  if (share.edge >= 0) edge = row.at(share.edge);
   Sums sum{neg_inf(), 0.f, 0.f};
-  for (int base = share.begin; base < share.end; base += kChunk) {
-    load_chunk<T, kThreads, kVecs>(row, share, base, r);
-    float top = Vec<T>::max(r[0]);
-#pragma unroll
-    for (int i = 1; i < kVecs; ++i) top = fmaxf(top, Vec<T>::max(r[i]));
-    accumulate<T, kVecs, true>(r, top, a.c, sum);
+#pragma unroll 1
+  for (int base = share.begin; base < share.end; base += cap) {
+    const int n = st.count(base, min(base + cap, share.end));
+    st.copy(row, base, n);
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      st.wait(q);
+      const int e = min(n, (q + 1) * st.per);
+#pragma unroll 1
+      for (int i = q * st.per; i < e; i += 2) {
+        uint4 r[2] = {st.buf[i * kThreads], neg_inf_vec<T>()};
+        if (i + 1 < e) r[1] = st.buf[(i + 1) * kThreads];
+        if (kMask) {
+          row.apply_mask(r[0], base + i * kThreads + Tm::tid());
+          st.buf[i * kThreads] = r[0];
+          if (i + 1 < e) {
+            row.apply_mask(r[1], base + (i + 1) * kThreads + Tm::tid());
+            st.buf[(i + 1) * kThreads] = r[1];
+          }
+        }
+        accumulate<T, 2, true>(r, a.c, sum);
+      }
+    }
   }
+  if (share.edge >= 0) sum = join(sum, single(edge, a.c), a.c);
   const float top = sum.m;
   sum = team_sums<kThreads>(sum, a.c, sh.red);
   int n = 0;
   if (o.top_k > 0)
-    n = collect_top<T, kThreads, kVecs>(row, share, r, top, o.top_k, sh.top);
+    n = collect_top<T, kThreads, kMask>(row, share, st, cap, edge, top, o.top_k, sh.top);
   const unsigned long long* keys = sh.top.cand;
   if (blocks > 1) {
     // the share's sums and its sorted top entries go to the first block
@@ -545,6 +615,7 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
     cluster_wait();
     if (rank != 0) return;
     sum = {cl.sums[0][0], cl.sums[0][1], cl.sums[0][2]};
+#pragma unroll 1
     for (int b = 1; b < blocks; ++b)
       sum = join(sum, Sums{cl.sums[b][0], cl.sums[b][1], cl.sums[b][2]}, a.c);
   }
@@ -559,6 +630,7 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
       o.stats[2 * row.index + 1] = s;
     }
   }
+#pragma unroll 1
   for (int k = Tm::tid(); k < o.n_targets; k += kThreads) {
     const long long i = o.targets[row.index * o.n_targets + k];
     float lp = 0.f;
@@ -584,34 +656,25 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
       if (at < o.top_k) put(at, keys[i]);
     }
     for (int i = n + Tm::tid(); i < o.top_k; i += kThreads) put(i, 0ull);
-  } else {
-    // each block's list is sorted: a key's place is its own plus the larger ones of the others
-    int total = 0;
-    for (int b = 0; b < blocks; ++b)
-      for (int i = Tm::tid(); i < o.top_k; i += kThreads) {
-        const unsigned long long key = cl.keys[b][i];
-        if (!key) continue;
-        int at = i;
-        for (int q = 0; q < blocks; ++q) {
-          if (q == b) continue;
-          int lo = 0, hi = o.top_k;                    // first place with a smaller key
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (cl.keys[q][mid] > key) lo = mid + 1; else hi = mid;
-          }
-          at += lo;
-        }
-        if (at < o.top_k) put(at, key);
-      }
-    for (int b = 0; b < blocks; ++b) {
-      int lo = 0, hi = o.top_k;
+    return;
+  }
+  // Each block's list is sorted: a key's place is its own plus the larger ones of the
+  // others. An empty place's key is 0; it ranks behind all others, by its list and place.
+  for (int i = Tm::tid(); i < blocks * o.top_k; i += kThreads) {
+    const int b = i / o.top_k;
+    const unsigned long long key = cl.keys[b][i - b * o.top_k];
+    int at = i - b * o.top_k;
+    for (int q = 0; q < blocks && at < o.top_k; ++q) {
+      if (q == b) continue;
+      int lo = 0, hi = o.top_k;                    // places with a larger key (empty: as large)
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (cl.keys[b][mid]) lo = mid + 1; else hi = mid;
+        if (cl.keys[q][mid] > key || (!key && (cl.keys[q][mid] || q < b))) lo = mid + 1;
+        else hi = mid;
       }
-      total += lo;
+      at += lo;
     }
-    for (int i = total + Tm::tid(); i < o.top_k; i += kThreads) put(i, 0ull);
+    if (at < o.top_k) put(at, key);
   }
 }
 
@@ -621,25 +684,24 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
 // the forward's m and s that is e (A + B x) for the first term: one
 // exponential and two products per entry, and no reduction over the row.
 // Dynamic shared memory: per team the spots' indices and gradients.
-template <typename T, int kThreads, int kVecs>
+template <typename T, int kThreads, bool kMask>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock)
 log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, unsigned rows,
                       int blocks) {
   using Tm = Team<kThreads>;
-  constexpr int N = Vec<T>::N, kChunk = kThreads * kVecs;
+  constexpr int N = Vec<T>::N, kVecs = 4;
   extern __shared__ int spots[];
   __shared__ float red[Tm::kPerBlock][Tm::kWarps];
   const unsigned r0 = blockIdx.x / blocks * Tm::kPerBlock + Tm::slot();
   if (kThreads == 32 && r0 >= rows) return;
   const Row<T> row(a, r0);
-  const Share share(row.nvec, blockIdx.x % blocks, blocks);
+  const Share<T> share(row, blockIdx.x % blocks, blocks, Tm::tid());
   const int nt = o.g_log_probs ? o.n_targets : 0, n = nt + (o.g_top ? o.top_k : 0);
   int* idx = spots + Tm::slot() * 2 * n;
   float* g = reinterpret_cast<float*>(idx + n);
-  uint4 r[kVecs];
-  if (share.begin < share.end) load_chunk<T, kThreads, kVecs>(row, share, share.begin, r);
   const float m = o.stats[2 * row.index], s = o.stats[2 * row.index + 1];
   float sum = 0.f;
+#pragma unroll 1
   for (int k = Tm::tid(); k < n; k += kThreads) {
     const bool given = k < nt;
     const long long i = given ? o.targets[row.index * o.n_targets + k]
@@ -667,68 +729,89 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
   const float f = s > 0.f ? a.inv_t / s : quiet_nan();
   const float A = f * (ac - gh * (h - logf(s))), B = -f * gh * kLn2;
   // A is NaN where the row has no distribution or no entry
-  auto value = [&](float z) {
-    const float x = fmaxf((z - m) * a.c, -1000.f);
-    return ex2(x) * fmaf(B, x, A);
+  const bool fine = A == A, vec_store = row.vec_store();
+  const f2 nm = {-m, -m}, cc = {a.c, a.c}, aa = {A, A}, bb = {B, B};
+  auto value = [&](f2 z) {
+    f2 x = mul2(add2(z, nm), cc);
+    x.x = fmaxf(x.x, -1000.f);
+    x.y = fmaxf(x.y, -1000.f);
+    return mul2(f2{ex2(x.x), ex2(x.y)}, fma2(bb, x, aa));
   };
-  for (int base = share.begin; base < share.end; base += kChunk) {
-    if (base != share.begin) load_chunk<T, kThreads, kVecs>(row, share, base, r);
+#pragma unroll 1
+  for (int j0 = share.begin + Tm::tid(); j0 < share.end; j0 += kVecs * kThreads) {
+    uint4 r[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (j0 + i * kThreads < share.end)
+        r[i] = __ldcs(reinterpret_cast<const uint4*>(row.vec(j0 + i * kThreads)));
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int j = base + i * kThreads + Tm::tid();
+      const int j = j0 + i * kThreads;
       if (j >= share.end) continue;
+      if (kMask) row.apply_mask(r[i], j);
       float z[N];
       Vec<T>::unpack(r[i], z);
-      if (A == A) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = value(z[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = z[e] == neg_inf() ? 0.f : A;
+      for (int e = 0; e < N; e += 2) {
+        f2 d = value(f2{z[e], z[e + 1]});
+        if (!fine) d = {z[e] == neg_inf() ? 0.f : A, z[e + 1] == neg_inf() ? 0.f : A};
+        z[e] = d.x;
+        z[e + 1] = d.y;
       }
-      row.store(j, z);
+      row.store(j, z, vec_store);
     }
   }
+  auto put = [&](int v, float more) {
+    const float z = row.at(v);
+    const float d = fmaf(more, a.inv_t, value(f2{z, z}).x);
+    row.grad[v] = to_type<T>(z == neg_inf() ? 0.f : fine ? d : A);
+  };
+  if (share.edge >= 0) put(share.edge, 0.f);
   if (n == 0) return;
   Tm::sync();                                     // the spots' entries are written again
+#pragma unroll 1
   for (int k = Tm::tid(); k < n; k += kThreads) {
-    const int v = idx[k], j = v < 0 ? -1 : (v + row.ph) / N;
-    if (j < share.begin || j >= share.end) continue;
+    const int v = idx[k];
+    if (v < share.first || v >= share.last) continue;
     bool first = true;
     for (int q = 0; q < k; ++q) first &= idx[q] != v;
     if (!first) continue;
     float at = 0.f;
     for (int q = k; q < n; ++q) at += idx[q] == v ? g[q] : 0.f;
-    const float z = row.at(v);
-    row.grad[v] = to_type<T>(z == neg_inf() ? 0.f : A == A ? fmaf(at, a.inv_t, value(z)) : A);
+    put(v, at);
   }
 }
 
 // ------------------------------------------------------------ distillation
-// Shared memory of one team, in this order (dynamic): p, logits, indices of
-// the list, and a bit per entry of the block's share (listed or not).
-__host__ __device__ constexpr int distill_bytes(int listed, int vecs, int n) {
-  return (16 * listed + ((vecs * n + 31) / 32) * 4 + 15) / 16 * 16;
+// Shared memory of one team, in this order (dynamic): the chunk; p, logits,
+// indices of the list; and a bit per entry of the block's share (listed or
+// not), from 32 places before its first vector to 32 behind its last.
+__host__ __device__ constexpr int distill_bytes(int listed, int cap, int vecs, int n) {
+  return cap * 16 + (16 * listed + (vecs * n / 32 + 3) * 4 + 15) / 16 * 16;
 }
 
-// Per warp: what the list adds up to, in 64 bits.
+static __device__ __noinline__ double exp64(double x) { return exp(x); }
+
+// Per warp: what the list adds up to.
 struct ListSums {
-  double mass, p_log_p, p_z, e;    // sum P, P log P, P z', 2^..: exp(z' - top)
+  double mass, p_log_p, p_z;       // sum P, P log P, P z' (relative to the largest z')
+  float e;                         // sum exp(z')
 };
 
 // The list's entries are dropped from the vectors before the one pass over
 // the row, so that pass gives maximum and sum over the rest alone, without a
-// difference of nearly equal numbers; the list itself is joined in 64 bits.
-// With lse_R, lse the logs of the two normalisers and q_R = exp(lse_R - lse)
+// difference of nearly equal numbers; the teacher's masses are added in 64
+// bits, for the rest's is 1 minus their sum. With lse_R, lse the logs of the
+// two normalisers and q_R = exp(lse_R - lse)
 //   dz_v = T w exp(z'_v - lse_R) (q_R - P_rest)     outside the list
 //   dz_u = T w (exp(z'_u - lse) - P_u)              in it
-// so the gradient is one more exponential per entry held in registers.
-template <typename T, int kThreads, int kVecs, int kMinBlocks>
-__global__ void __launch_bounds__(Team<kThreads>::kBlock, kMinBlocks)
+// so the gradient is one more exponential per entry in shared memory.
+template <typename T, int kThreads, bool kMask>
+__global__ void __launch_bounds__(Team<kThreads>::kBlock)
 distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned rows, int blocks,
-               int team_bytes) {
+               int cap, int team_bytes) {
   using Tm = Team<kThreads>;
-  constexpr int N = Vec<T>::N, kChunk = kThreads * kVecs;
+  constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Sums red[Tm::kPerBlock][Tm::kWarps];
   __shared__ ListSums lred[Tm::kPerBlock][Tm::kWarps];
@@ -741,34 +824,38 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   if (kThreads == 32 && r0 >= rows) return;
   if (blocks > 1) cluster_arrive();
   const Row<T> row(a, r0);
-  const Share share(row.nvec, rank, blocks);
-  double* p = reinterpret_cast<double*>(dyn + slot * team_bytes);
+  const Share<T> share(row, rank, blocks, Tm::tid());
+  unsigned char* mine = dyn + slot * team_bytes;
+  const Stage<T, kThreads> st(reinterpret_cast<uint4*>(mine), cap);
+  double* p = reinterpret_cast<double*>(mine + cap * 16);
   float* zu = reinterpret_cast<float*>(p + K);
   int* idx = reinterpret_cast<int*>(zu + K);
   uint32_t* bits = reinterpret_cast<uint32_t*>(idx + K);
+  const bool one = share.end - share.begin <= cap, vec_store = row.vec_store();
   float weight = o.weight ? o.weight[row.index] : 1.f;
-  const bool off = weight == 0.f;
-  weight *= o.scale;
-  if (o.upstream) weight *= o.upstream[row.index * o.upstream_stride];
-  if (off) {                                      // nothing of the row is looked at
+  st.copy(row, share.begin, st.count(share.begin, min(share.begin + cap, share.end)));
+  if (weight == 0.f) {                            // nothing of the row is looked at
+    cp_async_wait<0>();
     if (o.row_loss && rank == 0 && Tm::tid() == 0) o.row_loss[row.index] = 0.f;
     if (row.grad) {
       float zero[N];
 #pragma unroll
       for (int e = 0; e < N; ++e) zero[e] = 0.f;
-      for (int j = share.begin + Tm::tid(); j < share.end; j += kThreads) row.store(j, zero);
+      for (int j = share.begin + Tm::tid(); j < share.end; j += kThreads)
+        row.store(j, zero, vec_store);
+      if (share.edge >= 0) row.grad[share.edge] = to_type<T>(0.f);
     }
     if (blocks > 1) cluster_wait();
     return;
   }
-  uint4 r[kVecs];
-  if (share.begin < share.end) load_chunk<T, kThreads, kVecs>(row, share, share.begin, r);
-  const int words = ((share.end - share.begin) * N + 31) / 32;
+  weight *= o.scale;
+  if (o.upstream) weight *= o.upstream[row.index * o.upstream_stride];
+  // entry v has the bit v - v0
+  const int v0 = row.head + share.begin * N - 32, words = (share.end - share.begin) * N / 32 + 3;
   for (int w = Tm::tid(); w < words; w += kThreads) bits[w] = 0u;
-  Tm::sync();
   bool bad = false, twice = false;
   float top_lp = neg_inf(), top_z = neg_inf();
-  const int u0 = share.begin * N, u1 = share.end * N;
+#pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
     const long long i = o.indices[row.index * K + k];
     const float lp = o.log_probs[row.index * K + k];
@@ -783,18 +870,16 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       top_z = fmaxf(top_z, z);
     }
   }
-  // an entry in another block's share is marked there; repeats are looked for in order
   Tm::sync();
+#pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
     const int v = idx[k];
-    if (v < 0) continue;
-    const int u = v + row.ph;
-    if (u >= u0 && u < u1) {
-      const uint32_t old = atomicOr(&bits[(u - u0) >> 5], 1u << ((u - u0) & 31));
-      twice |= (old >> ((u - u0) & 31)) & 1u;
-    }
-    if (blocks > 1 && !twice)
+    if (v >= share.first && v < share.last) {
+      const uint32_t old = atomicOr(&bits[(v - v0) >> 5], 1u << ((v - v0) & 31));
+      twice |= (old >> ((v - v0) & 31)) & 1u;
+    } else if (v >= 0) {                          // repeats in the other blocks' shares
       for (int q = 0; q < k; ++q) twice |= idx[q] == v;
+    }
   }
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) {
@@ -808,20 +893,19 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     flags[slot][Tm::warp()] = flag;
   }
   Tm::sync();
+  const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
   int all = 0;
   top_lp = top_z = neg_inf();
-#pragma unroll
-  for (int w = 0; w < Tm::kWarps; ++w) {
+#pragma unroll 1
+  for (int w = 0; w < list_warps; ++w) {
     top_lp = fmaxf(top_lp, tops[slot][w][0]);
     top_z = fmaxf(top_z, tops[slot][w][1]);
     all |= flags[slot][w];
   }
   bad = all & 1;
-  const double t_ = a.t, inv_t = 1.0 / t_;
   const double shift = o.renormalize && top_lp > neg_inf() ? (double)top_lp : 0.0;
-  ListSums ls{0.0, 0.0, 0.0, 0.0};
   if (all & 2) {                                  // an entry listed twice counts once
-    for (int k = Tm::tid(); k < K; k += kThreads) p[k] = idx[k] < 0 ? 0.0 : exp(p[k] - shift);
+    for (int k = Tm::tid(); k < K; k += kThreads) p[k] = idx[k] < 0 ? 0.0 : exp64(p[k] - shift);
     Tm::sync();
     if (Tm::tid() == 0)
       for (int k = 0; k < K; ++k)
@@ -833,44 +917,72 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
           }
     Tm::sync();
   }
-  for (int k = Tm::tid(); k < K; k += kThreads) {
-    if (idx[k] < 0) continue;
-    const double lp = (all & 2) ? log(p[k]) : p[k] - shift;
-    const double pk = (all & 2) ? p[k] : exp(lp);
-    const double zp = ((double)zu[k] - (double)top_z) * inv_t;
-    p[k] = pk;
-    ls.mass += pk;
-    if (pk > 0.0) {
-      ls.p_log_p += pk * lp;
-      ls.p_z += pk * zp;
+  if (Tm::warp() < list_warps) {
+    ListSums ls{0.0, 0.0, 0.0, 0.f};
+#pragma unroll 1
+    for (int k = Tm::tid(); k < K; k += kThreads) {
+      if (idx[k] < 0) continue;
+      const double lp = (all & 2) ? log(p[k]) : p[k] - shift;
+      const double pk = (all & 2) ? p[k] : exp64(lp);
+      const float zp = (zu[k] - top_z) * a.inv_t;
+      p[k] = pk;
+      ls.mass += pk;
+      if (pk > 0.0) {
+        ls.p_log_p += pk * lp;
+        ls.p_z += pk * (double)zp;
+      }
+      ls.e += expf(zp);
     }
-    ls.e += exp(zp);
+#pragma unroll 1
+    for (int w = 16; w > 0; w >>= 1) {
+      ls.mass += __shfl_xor_sync(0xffffffffu, ls.mass, w);
+      ls.p_log_p += __shfl_xor_sync(0xffffffffu, ls.p_log_p, w);
+      ls.p_z += __shfl_xor_sync(0xffffffffu, ls.p_z, w);
+      ls.e += __shfl_xor_sync(0xffffffffu, ls.e, w);
+    }
+    if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
   }
   // the rest of the row
   Sums sum{neg_inf(), 0.f, 0.f};
-  for (int base = share.begin; base < share.end; base += kChunk) {
-    if (base != share.begin) load_chunk<T, kThreads, kVecs>(row, share, base, r);
-    float top = neg_inf();
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int j = base + i * kThreads + Tm::tid();
-      if (j >= share.end) continue;
-      const int u = j * N - u0;
-      const uint32_t b = (bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u);
-      if (b) drop_bits<T>(r[i], b);
-      top = fmaxf(top, Vec<T>::max(r[i]));
+  const int bit0 = Tm::tid() * N + 32;            // the thread's first bit in a chunk
+#pragma unroll 1
+  for (int base = share.begin; base < share.end; base += cap) {
+    const int n = st.count(base, min(base + cap, share.end));
+    if (base != share.begin) st.copy(row, base, n);
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      st.wait(q);
+      const int e = min(n, (q + 1) * st.per);
+#pragma unroll 1
+      for (int i = q * st.per; i < e; i += 2) {
+        uint4 r[2] = {st.buf[i * kThreads], neg_inf_vec<T>()};
+        if (i + 1 < e) r[1] = st.buf[(i + 1) * kThreads];
+        if (kMask) {
+          row.apply_mask(r[0], base + i * kThreads + Tm::tid());
+          st.buf[i * kThreads] = r[0];
+          if (i + 1 < e) {
+            row.apply_mask(r[1], base + (i + 1) * kThreads + Tm::tid());
+            st.buf[(i + 1) * kThreads] = r[1];
+          }
+        }
+        const int u = (base - share.begin + i * kThreads) * N + bit0;
+        const uint32_t b0 = (bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u);
+        if (b0) drop_bits<T>(r[0], b0);
+        if (i + 1 < e) {
+          const int u1 = u + kThreads * N;
+          const uint32_t b1 = (bits[u1 >> 5] >> (u1 & 31)) & ((1u << N) - 1u);
+          if (b1) drop_bits<T>(r[1], b1);
+        }
+        accumulate<T, 2, false>(r, a.c, sum);
+      }
     }
-    accumulate<T, kVecs, false>(r, top, a.c, sum);
   }
-  if (Tm::warp() * 32 < K)                        // the other warps have none of the list
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    ls.mass += __shfl_xor_sync(0xffffffffu, ls.mass, w);
-    ls.p_log_p += __shfl_xor_sync(0xffffffffu, ls.p_log_p, w);
-    ls.p_z += __shfl_xor_sync(0xffffffffu, ls.p_z, w);
-    ls.e += __shfl_xor_sync(0xffffffffu, ls.e, w);
+  float edge = neg_inf();
+  if (share.edge >= 0) {
+    edge = row.at(share.edge);
+    const int u = share.edge - v0;
+    if (!((bits[u >> 5] >> (u & 31)) & 1u)) sum = join(sum, single(edge, a.c), a.c);
   }
-  if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
   sum = team_sums<kThreads>(sum, a.c, red[slot]);   // orders lred, too (a barrier, or one warp)
   if constexpr (kThreads == 32) __syncwarp();
   if (blocks > 1) {
@@ -882,76 +994,93 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     cluster_arrive();
     cluster_wait();
     sum = {cl[0][0], cl[0][1], 0.f};
+#pragma unroll 1
     for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
   }
-  ls = lred[slot][0];
-#pragma unroll
-  for (int w = 1; w < Tm::kWarps; ++w) {
+  ListSums ls{0.0, 0.0, 0.0, 0.f};
+#pragma unroll 1
+  for (int w = 0; w < list_warps; ++w) {
     ls.mass += lred[slot][w].mass;
     ls.p_log_p += lred[slot][w].p_log_p;
     ls.p_z += lred[slot][w].p_z;
     ls.e += lred[slot][w].e;
   }
   const bool rest = sum.m != neg_inf(), listed = top_z != neg_inf();
-  bad |= sum.s != sum.s || ls.e != ls.e;
+  bad |= sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
   const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
   const double inv = whole && ls.mass > 0.0 ? 1.0 / ls.mass : 1.0;
-  const double p_r = whole ? 0.0 : 1.0 - ls.mass;
+  const float p_r = whole ? 0.f : (float)(1.0 - ls.mass);
   const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
-  // logs of the normalisers relative to the larger of the two maxima
-  const double big = fmaxf(rest ? sum.m : neg_inf(), top_z);
-  const double log_r = rest ? ((double)sum.m - big) * inv_t + log((double)sum.s) : 0.0;
-  const double lift = listed ? ((double)top_z - big) * inv_t : 0.0;
-  const double norm = (listed ? ls.e * exp(lift) : 0.0) + (rest ? exp(log_r) : 0.0);
-  const double log_all = log(norm);
+  // the two normalisers relative to the larger of the two maxima
+  const float big = fmaxf(rest ? sum.m : neg_inf(), top_z);
+  const float down_r = rest ? (sum.m - big) * a.inv_t : 0.f;
+  const float down_u = listed ? (top_z - big) * a.inv_t : 0.f;
+  const float norm_r = rest ? sum.s * expf(down_r) : 0.f;
+  const float norm = norm_r + (listed ? ls.e * expf(down_u) : 0.f);
+  const float log_all = logf(norm);
   if (rank == 0 && Tm::tid() == 0 && o.row_loss) {
     double loss = 0.0;
     if (live && ls.mass > 0.0)
-      loss = inv * (ls.p_log_p - ls.p_z + (log_all - lift) * ls.mass) + log(inv) * (inv * ls.mass);
-    if (p_r > 0.0) loss += p_r * (log(p_r) - (log_r - log_all));
-    if (!live) loss = 0.0;
-    o.row_loss[row.index] = bad ? quiet_nan() : (float)(loss * t_ * t_ * (double)weight);
+      loss = inv * (ls.p_log_p - ls.p_z + ((double)log_all - (double)down_u) * ls.mass) +
+             (whole ? log(inv) * (inv * ls.mass) : 0.0);
+    if (live && p_r > 0.f)
+      loss += (double)p_r * ((double)logf(p_r) -
+                             ((double)down_r + (double)logf(sum.s) - (double)log_all));
+    o.row_loss[row.index] =
+        bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
   }
   if (!row.grad) return;
-  const double q_r = rest ? exp(log_r - log_all) : 0.0, scale = (double)weight * t_;
-  const float coef = live && rest ? (float)(scale * (q_r - p_r) / (double)sum.s) : 0.f;
+  const float scale = weight * a.t;
+  const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
   const float ref = rest ? sum.m : 0.f, nan = quiet_nan();
   bad |= coef != coef;
-  for (int base = share.begin; base < share.end; base += kChunk) {
-    if (share.end - share.begin > kChunk) {
-      load_chunk<T, kThreads, kVecs>(row, share, base, r);
+  const f2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
+#pragma unroll 1
+  for (int base = share.begin; base < share.end; base += cap) {
+    const int n = st.count(base, min(base + cap, share.end));
+    if (!one) {
+      st.copy(row, base, n);
+      cp_async_wait<0>();
     }
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
       const int j = base + i * kThreads + Tm::tid();
-      if (j >= share.end) continue;
+      uint4 r = st.buf[i * kThreads];
+      if (kMask && !one) row.apply_mask(r, j);
       float z[N];
-      Vec<T>::unpack(r[i], z);
-      if (!bad) {
+      Vec<T>::unpack(r, z);
 #pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = ex2((z[e] - ref) * a.c) * coef;
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = z[e] == neg_inf() ? 0.f : nan;
+      for (int e = 0; e < N; e += 2) {
+        const f2 x = mul2(add2(f2{z[e], z[e + 1]}, nref), cc);
+        f2 d = mul2(f2{ex2(x.x), ex2(x.y)}, kk);
+        if (bad) d = {z[e] == neg_inf() ? 0.f : nan, z[e + 1] == neg_inf() ? 0.f : nan};
+        z[e] = d.x;
+        z[e + 1] = d.y;
       }
-      row.store(j, z);
+      row.store(j, z, vec_store);
     }
   }
+  if (share.edge >= 0)
+    row.grad[share.edge] =
+        to_type<T>(edge == neg_inf() ? 0.f : bad ? nan : ex2((edge - ref) * a.c) * coef);
   if (K == 0) return;
   Tm::sync();                                     // the listed entries are written again
+#pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
-    const int v = idx[k], u = v + row.ph;
-    if (v < 0 || u < u0 || u >= u1) continue;
-    const float q = expf((float)(((double)zu[k] - big) * inv_t - log_all));
-    const double d = live ? scale * ((double)q - p[k] * inv) : 0.0;
-    row.grad[v] = to_type<T>(bad ? nan : (float)d);
+    const int v = idx[k];
+    if (v < share.first || v >= share.last) continue;
+    const float q = expf((zu[k] - big) * a.inv_t) / norm;
+    const float d = live ? scale * (q - (float)(p[k] * inv)) : 0.f;
+    row.grad[v] = to_type<T>(bad ? nan : d);
   }
 }
 
 // Sum of the rows' losses by one block, in 64 bits and a fixed order.
 static __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* __restrict__ row_loss,
-                                                        long long n, float* __restrict__ loss) {
+                                                               long long n,
+                                                               float* __restrict__ loss) {
   __shared__ double red[32];
+  griddep_wait();
   double s = 0.0;
   for (long long i = threadIdx.x; i < n; i += blockDim.x) s += row_loss[i];
 #pragma unroll
