@@ -133,15 +133,6 @@ __device__ __forceinline__ uint4 neg_inf_vec() {
   return make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
 }
 
-// Packed fp32 pairs (two lanes per instruction).
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-  return *reinterpret_cast<f2*>(&r);
-}
-
 // One row of the launch. Whatever address it starts at, its entries are
 // `head` single ones up to a 16-byte boundary, nin full vectors, and a few
 // single ones behind; no access leaves the row.
@@ -256,9 +247,9 @@ constexpr int kMaxCluster = 8;
 template <typename T> struct Share {
   int begin, end, first, last;
   int edge;                        // this thread's single entry, or -1
-  __device__ __forceinline__ Share(const Row<T>& row, int rank, int blocks, int tid) {
+  __device__ __forceinline__ Share(const Row<T>& row, int rank, int log_blocks, int tid) {
     constexpr int N = Vec<T>::N;
-    const int per = (row.nin + blocks - 1) / blocks;
+    const int blocks = 1 << log_blocks, per = (row.nin + blocks - 1) >> log_blocks;
     begin = min(rank * per, row.nin);
     end = min(begin + per, row.nin);
     const int tail = row.head + row.nin * N;
@@ -322,14 +313,12 @@ __device__ __forceinline__ Sums single(float z, float c) {
   if (z == neg_inf()) return {z, 0.f, 0.f};
   return {z, ex2((z - z) * c), 0.f};              // NaN for NaN and +inf
 }
-// Adds vectors to the running sums: per entry one exponential, half an add, a
-// product and two sums each, and a clamp for the entropy's 0 * -inf.
+// Adds vectors, whose maximum is `top`, to the running sums: per entry one
+// exponential, half an add, a product and two sums each, and a clamp for the
+// entropy's 0 * -inf.
 template <typename T, int kVecs, bool kEntropy>
-__device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float c, Sums& a) {
+__device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float top, float c, Sums& a) {
   constexpr int N = Vec<T>::N;
-  float top = Vec<T>::max(r[0]);
-#pragma unroll
-  for (int i = 1; i < kVecs; ++i) top = fmaxf(top, Vec<T>::max(r[i]));
   if (top > a.m) {
     if (a.m != neg_inf()) {                       // else nothing to rescale yet
       const float d = fmaxf((a.m - top) * c, -1000.f), f = ex2(d);
@@ -338,22 +327,22 @@ __device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float c, Sum
     }
     a.m = top;
   }
-  const float ref = a.m == neg_inf() ? 0.f : a.m;
-  const f2 nref = {-ref, -ref}, cc = {c, c};
-  f2 s = {0.f, 0.f}, t = {0.f, 0.f};
+  const float ref = a.m == neg_inf() ? 0.f : -a.m;
+  const float2 nref = {ref, ref}, cc = {c, c};
+  float2 s = {0.f, 0.f}, t = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     float f[N];
     Vec<T>::unpack(r[i], f);
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
-      f2 x = mul2(add2(f2{f[e], f[e + 1]}, nref), cc);
-      const f2 p = {ex2(x.x), ex2(x.y)};
-      s = add2(s, p);
+      float2 x = __fmul2_rn(__fadd2_rn(float2{f[e], f[e + 1]}, nref), cc);
+      const float2 p = {ex2(x.x), ex2(x.y)};
+      s = __fadd2_rn(s, p);
       if (kEntropy) {
         x.x = fmaxf(x.x, -1000.f);
         x.y = fmaxf(x.y, -1000.f);
-        t = fma2(p, x, t);
+        t = __ffma2_rn(p, x, t);
       }
     }
   }
@@ -361,26 +350,6 @@ __device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float c, Sum
   if (kEntropy) a.t += t.x + t.y;
 }
 
-// Joins the team's sums (every thread gets the result).
-template <int kThreads>
-__device__ __forceinline__ Sums team_sums(Sums a, float c, Sums* red) {
-  using Tm = Team<kThreads>;
-#pragma unroll 1
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                 __shfl_xor_sync(0xffffffffu, a.t, o)};
-    a = join(a, b, c);
-  }
-  if constexpr (kThreads == 32) return a;
-  if (Tm::lane() == 0) red[Tm::warp()] = a;
-  __syncthreads();
-  a = red[0];
-#pragma unroll 1
-  for (int w = 1; w < Tm::kWarps; ++w) a = join(a, red[w], c);
-  return a;
-}
-
-// ------------------------------------------------------------ top entries
 // Order of the entries: larger logit first, then the lower index. A logit's
 // key is 0 where it has no probability.
 __device__ __forceinline__ uint32_t logit_key(float z) {
@@ -391,6 +360,68 @@ __device__ __forceinline__ uint32_t logit_key(float z) {
 __device__ __forceinline__ float key_logit(uint32_t b) {
   return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
+// Joins the team's sums (every thread gets the result): the maximum first, so
+// that each thread rescales its own sums once.
+template <int kThreads>
+__device__ __forceinline__ Sums team_sums(Sums a, float c, Sums* red) {
+  using Tm = Team<kThreads>;
+  const uint32_t top = __reduce_max_sync(0xffffffffu, logit_key(a.m));
+  const float m = top ? key_logit(top) : neg_inf();
+  const float d = fmaxf((a.m - m) * c, -1000.f), f = ex2(d);
+  a = {m, f * a.s, f * (a.t + d * a.s)};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+  }
+  if constexpr (kThreads == 32) return a;
+  if (Tm::lane() == 0) red[Tm::warp()] = a;
+  __syncthreads();
+  float all = red[0].m;
+#pragma unroll
+  for (int w = 1; w < Tm::kWarps; ++w) all = fmaxf(all, red[w].m);
+  Sums sum{all, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < Tm::kWarps; ++w) {
+    const Sums b = red[w];
+    const float db = fmaxf((b.m - all) * c, -1000.f), fb = ex2(db);
+    sum.s += fb * b.s;
+    sum.t += fb * (b.t + db * b.s);
+  }
+  return sum;
+}
+
+// A row that is read once goes through a ring of kBatches batches of four
+// vectors per thread: two batches are on their way while one is added up.
+constexpr int kBatch = 4, kBatches = 3, kSlots = kBatch * kBatches;
+
+template <typename T, int kThreads>
+struct Ring {
+  uint4* buf;                      // this thread's first slot
+  const T* src;                    // its next vector
+  int left;                        // vectors not yet asked for
+  int n;                           // vectors in all
+  __device__ __forceinline__ Ring(uint4* slots, const Row<T>& row, const Share<T>& share) {
+    buf = slots + Team<kThreads>::tid();
+    src = row.vec(share.begin + Team<kThreads>::tid());
+    n = left = max(0, share.end - share.begin - Team<kThreads>::tid() + kThreads - 1) / kThreads;
+  }
+  // asks for the next batch, into slots [slot, slot + 4); -inf behind the last vector
+  __device__ __forceinline__ void ask(int slot) {
+    if (left > 0) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (u < left) cp_async16(buf + (slot + u) * kThreads, src + u * kThreads * Vec<T>::N, true);
+        else buf[(slot + u) * kThreads] = neg_inf_vec<T>();
+      }
+      src += kBatch * kThreads * Vec<T>::N;
+      left -= kBatch;
+    }
+    cp_async_commit();
+  }
+};
+
+// ------------------------------------------------------------ top entries
 __device__ __forceinline__ unsigned long long order_key(uint32_t key, int v) {
   return ((unsigned long long)key << 32) | (0xffffffffu - (unsigned)v);
 }
@@ -398,70 +429,43 @@ __device__ __forceinline__ int key_index(unsigned long long key) {
   return (int)(0xffffffffu - (unsigned)key);
 }
 
-// Descending bitonic sort of one value per lane.
-__device__ __forceinline__ uint32_t warp_sort(uint32_t v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const uint32_t o = __shfl_xor_sync(0xffffffffu, v, j);
-      v = (((lane & j) == 0) == ((lane & k) == 0)) ? max(v, o) : min(v, o);
-    }
-  return v;
-}
-
-constexpr int kMaxCand = 512;      // entries that pass the bound of a block's top entries
-
 template <int kThreads> struct TopShared {
-  uint32_t sorted[Team<kThreads>::kWarps][32];
+  static constexpr int kMaxCand = 512;
   unsigned long long cand[kMaxCand];
+  uint32_t bound[Team<kThreads>::kWarps];
+  uint8_t list[Team<kThreads>::kWarps][32 * kBatch];
   int count;
   int red[Team<kThreads>::kWarps];
 };
 
-// Calls f(z, v) for this thread's entries of the share with z >= least (all,
-// where that is -inf), copying the chunks again if there are several.
+// Calls f(z, v) for this thread's entries of the share, read from memory.
 template <typename T, int kThreads, bool kMask, typename F>
-__device__ __forceinline__ void each_entry(const Row<T>& row, const Share<T>& share,
-                                           const Stage<T, kThreads>& st, int cap, float edge,
-                                           float least, F f) {
+__device__ __forceinline__ void each_entry(const Row<T>& row, const Share<T>& share, float edge,
+                                           F f) {
   constexpr int N = Vec<T>::N;
-  if (share.edge >= 0 && edge >= least) f(edge, share.edge);
+  if (share.edge >= 0) f(edge, share.edge);
 #pragma unroll 1
-  for (int base = share.begin; base < share.end; base += cap) {
-    const int n = st.count(base, min(base + cap, share.end));
-    if (share.end - share.begin > cap) {
-      st.copy(row, base, n);
-      cp_async_wait<0>();
-    }
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const int j = base + i * kThreads + Team<kThreads>::tid();
-      uint4 r = st.buf[i * kThreads];
-      if (kMask && share.end - share.begin > cap) row.apply_mask(r, j);
-      if (!(Vec<T>::max(r) >= least)) continue;
-      float z[N];
-      Vec<T>::unpack(r, z);
+  for (int j = share.begin + Team<kThreads>::tid(); j < share.end; j += kThreads) {
+    uint4 r = *reinterpret_cast<const uint4*>(row.vec(j));
+    if (kMask) row.apply_mask(r, j);
+    float z[N];
+    Vec<T>::unpack(r, z);
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (z[e] >= least) f(z[e], row.head + j * N + e);
-    }
+    for (int e = 0; e < N; ++e) f(z[e], row.head + j * N + e);
   }
 }
 
-// Rows that defeat the bound of collect_top (many equal logits, sorted rows)
-// are counted: bisection for the k-th largest logit, then for the index up to
+// Rows with more candidates than there is room for (many equal logits) are
+// counted: bisection for the k-th largest logit, then for the index up to
 // which its equals belong to the first k. Leaves exactly k candidates.
 template <typename T, int kThreads, bool kMask>
-__device__ __noinline__ int count_top(const Row<T>& row, const Share<T>& share,
-                                      const Stage<T, kThreads>& st, int cap, float edge,
+__device__ __noinline__ int count_top(const Row<T>& row, const Share<T>& share, float edge,
                                       uint32_t bound, int k, TopShared<kThreads>& sh) {
   using Tm = Team<kThreads>;
   // how many entries have a key of at least q (with `equal`: of exactly q, up to index v)
   auto count = [&](uint32_t q, bool equal, int last) {
     int n = 0;
-    each_entry<T, kThreads, kMask>(row, share, st, cap, edge, neg_inf(), [&](float z, int v) {
+    each_entry<T, kThreads, kMask>(row, share, edge, [&](float z, int v) {
       const uint32_t key = logit_key(z);
       n += equal ? key == q && v <= last : key >= q;
     });
@@ -481,7 +485,7 @@ __device__ __noinline__ int count_top(const Row<T>& row, const Share<T>& share,
   Tm::sync();
   if (Tm::tid() == 0) sh.count = 0;
   Tm::sync();
-  each_entry<T, kThreads, kMask>(row, share, st, cap, edge, neg_inf(), [&](float z, int v) {
+  each_entry<T, kThreads, kMask>(row, share, edge, [&](float z, int v) {
     const uint32_t key = logit_key(z);
     if (key > lo || (key == lo && v <= last)) sh.cand[atomicAdd(&sh.count, 1)] = order_key(key, v);
   });
@@ -489,40 +493,168 @@ __device__ __noinline__ int count_top(const Row<T>& row, const Share<T>& share,
   return sh.count;
 }
 
+// Drops candidates that are too many to be ranked one against all: the first
+// warp bisects over their logits until little more than k are left.
+template <int kThreads>
+__device__ __noinline__ int thin_out(int n, int k, TopShared<kThreads>& sh) {
+  using Tm = Team<kThreads>;
+  constexpr uint32_t kAll = 0xffffffffu;
+  if (Tm::warp() == 0) {
+    const int lane = Tm::lane();
+    uint32_t lo = 0, hi = kAll;
+    for (int left = n; hi - lo > 1 && left > k + k / 4;) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      int r = 0;
+      for (int i = lane; i < n; i += 32) r += (uint32_t)(sh.cand[i] >> 32) >= mid;
+      r = __reduce_add_sync(kAll, r);
+      if (r >= k) {
+        lo = mid;
+        left = r;
+      } else {
+        hi = mid;
+      }
+    }
+    int kept = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const unsigned long long key = i0 + lane < n ? sh.cand[i0 + lane] : 0ull;
+      const bool keep = key && (uint32_t)(key >> 32) >= lo;
+      const uint32_t vote = __ballot_sync(kAll, keep);
+      __syncwarp();
+      if (keep) sh.cand[kept + __popc(vote & ((1u << lane) - 1))] = key;
+      kept += __popc(vote);
+      __syncwarp();
+    }
+    if (lane == 0) sh.count = kept;
+  }
+  Tm::sync();
+  return sh.count;
+}
+
 // The k largest entries of a block's share and some more, in no order, into
 // sh.cand; returns their number (all there are if the share has fewer than k).
 //
-// Each thread knows the maximum of its entries. With the maxima of a warp
-// sorted, at least k entries reach the smallest over the warps of the
-// ceil(k / warps)-th, and k reach the k-th of any one warp; every entry at or
-// above the larger of the two is a candidate, on entries in no order about 2k
-// of them. Only threads whose maximum reaches the bound look again.
+// While the row passes, each thread keeps four maxima, one for every fourth of
+// its vectors: 4 * kThreads groups in all. If k of the groups have a maximum
+// of at least b, then k entries do, so every entry at or above b is a
+// candidate and only those groups are looked at again. b comes from bisection
+// over the maxima: in each warp for the ceil(k / warps)-th, and where the
+// warps differ too much (a profile's summit lies in few of them) over all.
 template <typename T, int kThreads, bool kMask>
 __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& share,
-                                           const Stage<T, kThreads>& st, int cap, float edge,
-                                           float top, int k, TopShared<kThreads>& sh) {
+                                           const Ring<T, kThreads>& ring, float edge,
+                                           const float (&top)[kBatch], int k,
+                                           TopShared<kThreads>& sh) {
   using Tm = Team<kThreads>;
-  if (Tm::tid() == 0) sh.count = 0;
-  sh.sorted[Tm::warp()][Tm::lane()] = warp_sort(logit_key(top));
-  Tm::sync();
-  const int each = (k + Tm::kWarps - 1) / Tm::kWarps;
-  uint32_t low = 0xffffffffu, high = 0u;
+  constexpr int N = Vec<T>::N;
+  constexpr uint32_t kAll = 0xffffffffu;
+  uint32_t key[kBatch], most = 0;
 #pragma unroll
-  for (int w = 0; w < Tm::kWarps; ++w) {
-    low = min(low, each <= 32 ? sh.sorted[w][each - 1] : 0u);
-    high = max(high, k <= 32 ? sh.sorted[w][k - 1] : 0u);
+  for (int u = 0; u < kBatch; ++u) {
+    key[u] = logit_key(top[u]);
+    most = max(most, key[u]);
   }
-  const uint32_t bound = max(low, high);
-  const float least = bound ? key_logit(bound) : -3.4028234664e38f;   // the lowest logit there is
-  if (!(top < least))
-    each_entry<T, kThreads, kMask>(row, share, st, cap, edge, least, [&](float z, int v) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kMaxCand) sh.cand[at] = order_key(logit_key(z), v);
-    });
+  auto reach = [&](uint32_t q) {
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) n += key[u] >= q;
+    return n;
+  };
+  const int want = (k + Tm::kWarps - 1) / Tm::kWarps;
+  // 32 maxima reach the smallest of the lanes' largest
+  uint32_t lo = want <= 32 ? __reduce_min_sync(kAll, most) : 0u;
+  uint32_t hi = __reduce_max_sync(kAll, most) + 1;
+  for (int n = 128; hi - lo > 1 && n > want + want / 4;) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const int r = __reduce_add_sync(kAll, reach(mid));
+    if (r >= want) {
+      lo = mid;
+      n = r;
+    } else {
+      hi = mid;
+    }
+  }
+  if (Tm::tid() == 0) sh.count = 0;
+  if constexpr (Tm::kWarps > 1) {
+    if (Tm::lane() == 0) sh.bound[Tm::warp()] = lo;
+    __syncthreads();
+    uint32_t up = 0;
+#pragma unroll
+    for (int w = 0; w < Tm::kWarps; ++w) {
+      lo = min(lo, sh.bound[w]);
+      up = max(up, sh.bound[w]);
+    }
+    for (int n = Tm::sum(reach(lo), sh.red); up - lo > 1 && n > 2 * k + 16;) {
+      const uint32_t mid = lo + (up - lo) / 2;
+      const int r = Tm::sum(reach(mid), sh.red);
+      if (r >= k) {
+        lo = mid;
+        n = r;
+      } else {
+        up = mid;
+      }
+    }
+  }
+  const float least = lo ? key_logit(lo) : -3.4028234664e38f;   // the lowest logit there is
+  // the groups that reach it, warp by warp: their vectors, one to a lane
+  uint8_t* list = sh.list[Tm::warp()];
+  int groups = 0;
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    const bool in = top[u] >= least;
+    const uint32_t vote = __ballot_sync(kAll, in);
+    if (in) list[groups + __popc(vote & ((1u << Tm::lane()) - 1))] = Tm::lane() * kBatch + u;
+    groups += __popc(vote);
+  }
+  __syncwarp();                                        // and the copies of the other lanes
+  auto push = [&](float z, int v) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < TopShared<kThreads>::kMaxCand) sh.cand[at] = order_key(logit_key(z), v);
+  };
+  if (share.edge >= 0 && edge >= least) push(edge, share.edge);
+  const int len = share.end - share.begin;
+  const int per = (len + kBatch * kThreads - 1) / (kBatch * kThreads);   // vectors of a group
+  const bool here = len <= kSlots * kThreads;          // the ring still holds the row
+  const int items = groups * per;
+  const uint4* slots = ring.buf - Tm::tid() + Tm::warp() * 32;
+#pragma unroll 1
+  for (int t0 = Tm::lane(); t0 < items; t0 += 32 * kBatch) {
+    uint4 r[kBatch];
+    int j[kBatch];
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int t = t0 + 32 * x, g = t / per;
+      j[x] = -1;
+      r[x] = neg_inf_vec<T>();
+      if (t < items) {
+        const int who = list[g], i = (t - g * per) * kBatch + (who & (kBatch - 1));
+        j[x] = share.begin + i * kThreads + Tm::warp() * 32 + who / kBatch;
+        if (j[x] < share.end)
+          r[x] = here ? slots[i * kThreads + who / kBatch]
+                      : __ldg(reinterpret_cast<const uint4*>(row.vec(j[x])));
+      }
+    }
+#pragma unroll 1
+    for (int x = 0; x < kBatch; ++x) {
+      uint4 q = r[0];
+      if (x == 1) q = r[1];
+      if (x == 2) q = r[2];
+      if (x == 3) q = r[3];
+      const int jx = x == 0 ? j[0] : x == 1 ? j[1] : x == 2 ? j[2] : j[3];
+      if (jx < 0 || jx >= share.end) continue;
+      if (kMask && !here) row.apply_mask(q, jx);
+      if (!(Vec<T>::max(q) >= least)) continue;
+      float z[N];
+      Vec<T>::unpack(q, z);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (z[e] >= least) push(z[e], row.head + jx * N + e);
+    }
+  }
   Tm::sync();
   const int n = sh.count;
-  if (n <= kMaxCand) return n;
-  return count_top<T, kThreads, kMask>(row, share, st, cap, edge, bound, k, sh);
+  if (n <= 2 * k + 16) return n;
+  if (n <= TopShared<kThreads>::kMaxCand) return thin_out<kThreads>(n, k, sh);
+  return count_top<T, kThreads, kMask>(row, share, edge, lo, k, sh);
 }
 
 // Place of a key among `n` different ones, the largest first.
@@ -545,59 +677,63 @@ struct ScoreCluster {
   unsigned long long keys[kMaxCluster][kMaxTop];
 };
 
-// One pass over the row for maximum, sum and entropy; the top entries from
-// the row in shared memory; the given entries by a gather at the end.
-// Dynamic shared memory: per team `cap` vectors; ScoreCluster if blocks > 1.
+// One pass over the row for maximum, sum, entropy and the groups' maxima; the
+// top entries from the groups that matter; the given entries by a gather at
+// the end. Dynamic shared memory: per team a ring; ScoreCluster if blocks > 1.
 template <typename T, int kThreads, bool kMask>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock)
-log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned rows, int blocks,
-                 int cap) {
+log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned rows, int log_blocks) {
   using Tm = Team<kThreads>;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ ScoreShared<kThreads> shared[Tm::kPerBlock];
   ScoreShared<kThreads>& sh = shared[Tm::slot()];
-  uint4* chunk = reinterpret_cast<uint4*>(dyn) + Tm::slot() * cap;
-  ScoreCluster& cl = *reinterpret_cast<ScoreCluster*>(dyn + cap * 16);
-  const unsigned r0 = blockIdx.x / blocks * Tm::kPerBlock + Tm::slot();
-  const int rank = blockIdx.x % blocks;
+  uint4* slots = reinterpret_cast<uint4*>(dyn) + Tm::slot() * kSlots * kThreads;
+  ScoreCluster& cl = *reinterpret_cast<ScoreCluster*>(dyn + kSlots * kThreads * 16);
+  const int blocks = 1 << log_blocks, rank = blockIdx.x & (blocks - 1);
+  const unsigned r0 = (blockIdx.x >> log_blocks) * Tm::kPerBlock + Tm::slot();
   if (kThreads == 32 && r0 >= rows) return;            // a whole warp, and no cluster
   if (blocks > 1) cluster_arrive();                    // the blocks of the cluster have begun
   const Row<T> row(a, r0);
-  const Share<T> share(row, rank, blocks, Tm::tid());
-  const Stage<T, kThreads> st(chunk, cap);
+  const Share<T> share(row, rank, log_blocks, Tm::tid());
+  Ring<T, kThreads> ring(slots, row, share);
+  ring.ask(0);
+  ring.ask(kBatch);
   float edge = neg_inf();
   if (share.edge >= 0) edge = row.at(share.edge);
-  Sums sum{neg_inf(), 0.f, 0.f};
+  Sums sum = single(edge, a.c);
+  float top[kBatch];
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) top[u] = neg_inf();
+  int slot = 0;
 #pragma unroll 1
-  for (int base = share.begin; base < share.end; base += cap) {
-    const int n = st.count(base, min(base + cap, share.end));
-    st.copy(row, base, n);
-#pragma unroll 1
-    for (int q = 0; q < 4; ++q) {
-      st.wait(q);
-      const int e = min(n, (q + 1) * st.per);
-#pragma unroll 1
-      for (int i = q * st.per; i < e; i += 2) {
-        uint4 r[2] = {st.buf[i * kThreads], neg_inf_vec<T>()};
-        if (i + 1 < e) r[1] = st.buf[(i + 1) * kThreads];
-        if (kMask) {
-          row.apply_mask(r[0], base + i * kThreads + Tm::tid());
-          st.buf[i * kThreads] = r[0];
-          if (i + 1 < e) {
-            row.apply_mask(r[1], base + (i + 1) * kThreads + Tm::tid());
-            st.buf[(i + 1) * kThreads] = r[1];
-          }
+  for (int i = 0; i < ring.n; i += kBatch) {
+    cp_async_wait<kBatches - 2>();
+    uint4 r[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) r[u] = ring.buf[(slot + u) * kThreads];
+    ring.ask(slot >= kBatch ? slot - kBatch : slot + (kBatches - 1) * kBatch);
+    if (kMask) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i + u < ring.n) {
+          row.apply_mask(r[u], share.begin + (i + u) * kThreads + Tm::tid());
+          ring.buf[(slot + u) * kThreads] = r[u];
         }
-        accumulate<T, 2, true>(r, a.c, sum);
-      }
     }
+    slot = slot == (kBatches - 1) * kBatch ? 0 : slot + kBatch;
+    float all = neg_inf();
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float t = Vec<T>::max(r[u]);
+      top[u] = fmaxf(top[u], t);
+      all = fmaxf(all, t);
+    }
+    accumulate<T, kBatch, true>(r, all, a.c, sum);
   }
-  if (share.edge >= 0) sum = join(sum, single(edge, a.c), a.c);
-  const float top = sum.m;
+  cp_async_wait<0>();
   sum = team_sums<kThreads>(sum, a.c, sh.red);
   int n = 0;
-  if (o.top_k > 0)
-    n = collect_top<T, kThreads, kMask>(row, share, st, cap, edge, top, o.top_k, sh.top);
+  if (o.top_k > 0) n = collect_top<T, kThreads, kMask>(row, share, ring, edge, top, o.top_k, sh.top);
   const unsigned long long* keys = sh.top.cand;
   if (blocks > 1) {
     // the share's sums and its sorted top entries go to the first block
@@ -678,6 +814,23 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
   }
 }
 
+// The gradient of a row without a distribution: NaN, and 0 where an entry does
+// not take part.
+template <typename T, int kThreads, bool kMask>
+__device__ __noinline__ void fill_bad(const Row<T>& row, const Share<T>& share) {
+  constexpr int N = Vec<T>::N;
+#pragma unroll 1
+  for (int j = share.begin + Team<kThreads>::tid(); j < share.end; j += kThreads) {
+    uint4 r = *reinterpret_cast<const uint4*>(row.vec(j));
+    if (kMask) row.apply_mask(r, j);
+    float z[N];
+    Vec<T>::unpack(r, z);
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e] = z[e] == neg_inf() ? 0.f : quiet_nan();
+    row.store(j, z, false);
+  }
+}
+
 // ------------------------------------------------------- and their gradient
 // dz_v = (q_v (a - g_H (log q_v + H)) + sum of the incoming gradients at v) / T
 // with a = g_norm - the sum of all incoming gradients of single entries. With
@@ -687,15 +840,15 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
 template <typename T, int kThreads, bool kMask>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock)
 log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, unsigned rows,
-                      int blocks) {
+                      int log_blocks) {
   using Tm = Team<kThreads>;
   constexpr int N = Vec<T>::N, kVecs = 4;
   extern __shared__ int spots[];
   __shared__ float red[Tm::kPerBlock][Tm::kWarps];
-  const unsigned r0 = blockIdx.x / blocks * Tm::kPerBlock + Tm::slot();
+  const unsigned r0 = (blockIdx.x >> log_blocks) * Tm::kPerBlock + Tm::slot();
   if (kThreads == 32 && r0 >= rows) return;
   const Row<T> row(a, r0);
-  const Share<T> share(row, blockIdx.x % blocks, blocks, Tm::tid());
+  const Share<T> share(row, blockIdx.x & ((1 << log_blocks) - 1), log_blocks, Tm::tid());
   const int nt = o.g_log_probs ? o.n_targets : 0, n = nt + (o.g_top ? o.top_k : 0);
   int* idx = spots + Tm::slot() * 2 * n;
   float* g = reinterpret_cast<float*>(idx + n);
@@ -730,41 +883,44 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
   const float A = f * (ac - gh * (h - logf(s))), B = -f * gh * kLn2;
   // A is NaN where the row has no distribution or no entry
   const bool fine = A == A, vec_store = row.vec_store();
-  const f2 nm = {-m, -m}, cc = {a.c, a.c}, aa = {A, A}, bb = {B, B};
-  auto value = [&](f2 z) {
-    f2 x = mul2(add2(z, nm), cc);
+  const float2 nm = {-m, -m}, cc = {a.c, a.c}, aa = {A, A}, bb = {B, B};
+  auto value = [&](float2 z) {
+    float2 x = __fmul2_rn(__fadd2_rn(z, nm), cc);
     x.x = fmaxf(x.x, -1000.f);
     x.y = fmaxf(x.y, -1000.f);
-    return mul2(f2{ex2(x.x), ex2(x.y)}, fma2(bb, x, aa));
+    return __fmul2_rn(float2{ex2(x.x), ex2(x.y)}, __ffma2_rn(bb, x, aa));
   };
+  if (fine) {
 #pragma unroll 1
-  for (int j0 = share.begin + Tm::tid(); j0 < share.end; j0 += kVecs * kThreads) {
-    uint4 r[kVecs];
+    for (int j0 = share.begin + Tm::tid(); j0 < share.end; j0 += kVecs * kThreads) {
+      uint4 r[kVecs];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (j0 + i * kThreads < share.end)
-        r[i] = __ldcs(reinterpret_cast<const uint4*>(row.vec(j0 + i * kThreads)));
+      for (int i = 0; i < kVecs; ++i)
+        if (j0 + i * kThreads < share.end)
+          r[i] = __ldcs(reinterpret_cast<const uint4*>(row.vec(j0 + i * kThreads)));
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int j = j0 + i * kThreads;
-      if (j >= share.end) continue;
-      if (kMask) row.apply_mask(r[i], j);
-      float z[N];
-      Vec<T>::unpack(r[i], z);
+      for (int i = 0; i < kVecs; ++i) {
+        const int j = j0 + i * kThreads;
+        if (j >= share.end) break;
+        if (kMask) row.apply_mask(r[i], j);
+        float z[N];
+        Vec<T>::unpack(r[i], z);
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        f2 d = value(f2{z[e], z[e + 1]});
-        if (!fine) d = {z[e] == neg_inf() ? 0.f : A, z[e + 1] == neg_inf() ? 0.f : A};
-        z[e] = d.x;
-        z[e + 1] = d.y;
+        for (int e = 0; e < N; e += 2) {
+          const float2 d = value(float2{z[e], z[e + 1]});
+          z[e] = d.x;
+          z[e + 1] = d.y;
+        }
+        row.store(j, z, vec_store);
       }
-      row.store(j, z, vec_store);
     }
+  } else {
+    fill_bad<T, kThreads, kMask>(row, share);
   }
   auto put = [&](int v, float more) {
     const float z = row.at(v);
-    const float d = fmaf(more, a.inv_t, value(f2{z, z}).x);
-    row.grad[v] = to_type<T>(z == neg_inf() ? 0.f : fine ? d : A);
+    const float d = fmaf(more, a.inv_t, value(float2{z, z}).x);
+    row.grad[v] = to_type<T>(z == neg_inf() ? 0.f : fine ? d : quiet_nan());
   };
   if (share.edge >= 0) put(share.edge, 0.f);
   if (n == 0) return;
@@ -808,7 +964,7 @@ struct ListSums {
 // so the gradient is one more exponential per entry in shared memory.
 template <typename T, int kThreads, bool kMask>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock)
-distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned rows, int blocks,
+distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned rows, int log_blocks,
                int cap, int team_bytes) {
   using Tm = Team<kThreads>;
   constexpr int N = Vec<T>::N;
@@ -819,12 +975,12 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   __shared__ int flags[Tm::kPerBlock][Tm::kWarps];
   __shared__ float cl[kMaxCluster][2];            // every block's maximum and sum
   const int slot = Tm::slot(), K = o.n_listed;
-  const unsigned r0 = blockIdx.x / blocks * Tm::kPerBlock + slot;
-  const int rank = blockIdx.x % blocks;
+  const int blocks = 1 << log_blocks, rank = blockIdx.x & (blocks - 1);
+  const unsigned r0 = (blockIdx.x >> log_blocks) * Tm::kPerBlock + slot;
   if (kThreads == 32 && r0 >= rows) return;
   if (blocks > 1) cluster_arrive();
   const Row<T> row(a, r0);
-  const Share<T> share(row, rank, blocks, Tm::tid());
+  const Share<T> share(row, rank, log_blocks, Tm::tid());
   unsigned char* mine = dyn + slot * team_bytes;
   const Stage<T, kThreads> st(reinterpret_cast<uint4*>(mine), cap);
   double* p = reinterpret_cast<double*>(mine + cap * 16);
@@ -973,7 +1129,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
           const uint32_t b1 = (bits[u1 >> 5] >> (u1 & 31)) & ((1u << N) - 1u);
           if (b1) drop_bits<T>(r[1], b1);
         }
-        accumulate<T, 2, false>(r, a.c, sum);
+        accumulate<T, 2, false>(r, fmaxf(Vec<T>::max(r[0]), Vec<T>::max(r[1])), a.c, sum);
       }
     }
   }
@@ -1034,31 +1190,34 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
   const float ref = rest ? sum.m : 0.f, nan = quiet_nan();
   bad |= coef != coef;
-  const f2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
+  const float2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
+  if (!bad) {
 #pragma unroll 1
-  for (int base = share.begin; base < share.end; base += cap) {
-    const int n = st.count(base, min(base + cap, share.end));
-    if (!one) {
-      st.copy(row, base, n);
-      cp_async_wait<0>();
-    }
-#pragma unroll 2
-    for (int i = 0; i < n; ++i) {
-      const int j = base + i * kThreads + Tm::tid();
-      uint4 r = st.buf[i * kThreads];
-      if (kMask && !one) row.apply_mask(r, j);
-      float z[N];
-      Vec<T>::unpack(r, z);
-#pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        const f2 x = mul2(add2(f2{z[e], z[e + 1]}, nref), cc);
-        f2 d = mul2(f2{ex2(x.x), ex2(x.y)}, kk);
-        if (bad) d = {z[e] == neg_inf() ? 0.f : nan, z[e + 1] == neg_inf() ? 0.f : nan};
-        z[e] = d.x;
-        z[e + 1] = d.y;
+    for (int base = share.begin; base < share.end; base += cap) {
+      const int n = st.count(base, min(base + cap, share.end));
+      if (!one) {
+        st.copy(row, base, n);
+        cp_async_wait<0>();
       }
-      row.store(j, z, vec_store);
+#pragma unroll 2
+      for (int i = 0; i < n; ++i) {
+        const int j = base + i * kThreads + Tm::tid();
+        uint4 r = st.buf[i * kThreads];
+        if (kMask && !one) row.apply_mask(r, j);
+        float z[N];
+        Vec<T>::unpack(r, z);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const float2 x = __fmul2_rn(__fadd2_rn(float2{z[e], z[e + 1]}, nref), cc);
+          const float2 d = __fmul2_rn(float2{ex2(x.x), ex2(x.y)}, kk);
+          z[e] = d.x;
+          z[e + 1] = d.y;
+        }
+        row.store(j, z, vec_store);
+      }
     }
+  } else {
+    fill_bad<T, kThreads, kMask>(row, share);
   }
   if (share.edge >= 0)
     row.grad[share.edge] =

@@ -12,10 +12,10 @@ namespace chm {
 namespace lk {
 namespace {
 
-// How a launch is cut: threads of a team, blocks of a row's cluster, and the
-// vectors of a block's chunk (a multiple of the threads).
+// How a launch is cut: threads of a team, blocks of a row's cluster (a power
+// of two), and the vectors of a block's chunk (a multiple of the threads).
 struct Cut {
-  int threads, blocks, cap;
+  int threads, log_blocks, cap;
 };
 
 int largest(const Rows& a) { return *std::max_element(a.size, a.size + a.ng); }
@@ -26,22 +26,32 @@ int largest(const Rows& a) { return *std::max_element(a.size, a.size + a.ng); }
 constexpr int kChunkBytes = 96 << 10;
 Cut cut_rows(int nvec, long long rows, bool warp) {
   Cut c{};
-  c.blocks = 1;
-  while (c.blocks < kMaxCluster && nvec > c.blocks * (kChunkBytes / 16)) c.blocks *= 2;
-  while (c.blocks < kMaxCluster && rows * c.blocks < 2 * 148 && nvec > c.blocks * 512)
-    c.blocks *= 2;
-  const int share = (nvec + c.blocks - 1) / c.blocks;
+  while (c.log_blocks < 3 && nvec > (kChunkBytes / 16) << c.log_blocks) ++c.log_blocks;
+  while (c.log_blocks < 3 && rows << c.log_blocks < 2 * 148 && nvec > 512 << c.log_blocks)
+    ++c.log_blocks;
+  const int share = (nvec + (1 << c.log_blocks) - 1) >> c.log_blocks;
   c.threads = warp && share <= 64 ? 32 : share <= 1024 ? 128 : share <= 4096 ? 256 : 512;
-  if (c.blocks > 1 && c.threads < 256) c.threads = 256;
+  if (c.log_blocks && c.threads < 256) c.threads = 256;
   const int most = std::min(std::max(share, 1), kChunkBytes / 16);
   c.cap = (most + c.threads - 1) / c.threads * c.threads;
   return c;
 }
 
+// For the kernels that read a row once, a warp up to 16 vectors a lane, else a
+// block of 128, of which several share a row where there are few.
+Cut cut_stream(int nvec, long long rows, int top_k) {
+  Cut c{};
+  c.threads = nvec <= 512 && top_k <= 64 ? 32 : 128;
+  if (c.threads == 128)
+    while (c.log_blocks < 3 && rows << c.log_blocks < 6 * 148 && nvec > 1024 << c.log_blocks)
+      ++c.log_blocks;
+  return c;
+}
+
 template <typename... KArgs, typename... Args>
-int launch(void (*kernel)(KArgs...), int threads, int blocks, long long rows, size_t smem,
+int launch(void (*kernel)(KArgs...), int threads, int log_blocks, long long rows, size_t smem,
            cudaStream_t st, bool cluster, Args... args) {
-  const int per_block = threads == 32 ? 4 : 1;
+  const int per_block = threads == 32 ? 4 : 1, blocks = 1 << log_blocks;
   const long long grid = (rows + per_block - 1) / per_block * blocks;
   if (grid > INT_MAX) return CHM_ERR_UNSUPPORTED;
   if (smem > 32 << 10 &&
@@ -68,19 +78,14 @@ int launch(void (*kernel)(KArgs...), int threads, int blocks, long long rows, si
 
 template <typename T, bool kMask>
 int run_log_probs_m(const Rows& a, const ScoreArgs& o, long long n, cudaStream_t st) {
-  const Cut c = cut_rows(largest(a) / Vec<T>::N, n, o.top_k <= 8);
-  const size_t smem = (size_t)(c.threads == 32 ? 4 : 1) * c.cap * 16 +
-                      (c.blocks > 1 ? sizeof(ScoreCluster) : 0);
+  const Cut c = cut_stream(largest(a) / Vec<T>::N, n, o.top_k);
+  const size_t smem = (size_t)kSlots * 128 * 16 + (c.log_blocks ? sizeof(ScoreCluster) : 0);
   auto run = [&](auto kernel) {
-    return launch(kernel, c.threads, c.blocks, n, smem, st, true, a, o, (unsigned)n, c.blocks,
-                  c.cap);
+    return launch(kernel, c.threads, c.log_blocks, n, smem, st, true, a, o, (unsigned)n,
+                  c.log_blocks);
   };
-  switch (c.threads) {
-    case 32: return run(log_probs_kernel<T, 32, kMask>);
-    case 128: return run(log_probs_kernel<T, 128, kMask>);
-    case 256: return run(log_probs_kernel<T, 256, kMask>);
-    default: return run(log_probs_kernel<T, 512, kMask>);
-  }
+  return c.threads == 32 ? run(log_probs_kernel<T, 32, kMask>)
+                         : run(log_probs_kernel<T, 128, kMask>);
 }
 
 template <typename T>
@@ -91,12 +96,14 @@ int run_log_probs(const Rows& a, const ScoreArgs& o, long long n, cudaStream_t s
 template <typename T, bool kMask>
 int run_log_probs_grad_m(const Rows& a, const ScoreGradArgs& o, long long n, cudaStream_t st) {
   const int nvec = largest(a) / Vec<T>::N;
-  // no exchange between blocks: long rows are cut into blocks of 256 x 16 vectors
-  const int threads = nvec <= 256 ? 32 : 256, blocks = threads == 32 ? 1 : (nvec + 4095) / 4096;
+  // no exchange between blocks: long rows are cut into blocks of at most 256 x 16 vectors
+  const int threads = nvec <= 256 ? 32 : 256;
+  int log_blocks = 0;
+  while (threads == 256 && nvec > 4096 << log_blocks) ++log_blocks;
   const int spots = o.n_targets * (o.g_log_probs != nullptr) + o.top_k * (o.g_top != nullptr);
   const size_t smem = (size_t)(threads == 32 ? 4 : 1) * spots * 8;
   auto run = [&](auto kernel) {
-    return launch(kernel, threads, blocks, n, smem, st, false, a, o, (unsigned)n, blocks);
+    return launch(kernel, threads, log_blocks, n, smem, st, false, a, o, (unsigned)n, log_blocks);
   };
   return threads == 32 ? run(log_probs_grad_kernel<T, 32, kMask>)
                        : run(log_probs_grad_kernel<T, 256, kMask>);
@@ -113,11 +120,11 @@ int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t
   const int nvec = largest(a) / Vec<T>::N;
   const Cut c = cut_rows(nvec, n, o.n_listed <= 128);
   const int team =
-      distill_bytes(o.n_listed, c.cap, (nvec + c.blocks - 1) / c.blocks, Vec<T>::N);
+      distill_bytes(o.n_listed, c.cap, (nvec >> c.log_blocks) + 1, Vec<T>::N);
   const size_t smem = (size_t)(c.threads == 32 ? 4 : 1) * team;
   auto run = [&](auto kernel) {
-    return launch(kernel, c.threads, c.blocks, n, smem, st, true, a, o, (unsigned)n, c.blocks,
-                  c.cap, team);
+    return launch(kernel, c.threads, c.log_blocks, n, smem, st, true, a, o, (unsigned)n,
+                  c.log_blocks, c.cap, team);
   };
   switch (c.threads) {
     case 32: return run(distill_kernel<T, 32, kMask>);
