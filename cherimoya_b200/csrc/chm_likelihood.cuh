@@ -133,6 +133,63 @@ __device__ __forceinline__ uint4 neg_inf_vec() {
   return make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
 }
 
+// Shared memory by 32-bit address plus an offset known at compile time.
+template <int kOff> __device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(a), "n"(kOff)
+               : "memory");
+  return r;
+}
+template <int kOff> __device__ __forceinline__ void sts128(uint32_t a, const uint4& r) {
+  asm volatile("st.shared.v4.u32 [%0 + %1], {%2, %3, %4, %5};" ::"r"(a), "n"(kOff), "r"(r.x),
+               "r"(r.y), "r"(r.z), "r"(r.w)
+               : "memory");
+}
+template <int kSOff, int kGOff>
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %1], [%2 + %3], 16;" ::"r"(dst), "n"(kSOff),
+               "l"(src), "n"(kGOff)
+               : "memory");
+}
+
+constexpr int kBatch = 4;          // vectors that a thread takes at a time
+
+// A thread's next kBatch vectors of a row to a place in shared memory, both
+// kStride vectors apart; -inf for those behind its last.
+template <typename T, int kStride>
+__device__ __forceinline__ void copy_batch(uint32_t dst, const char* src, int left) {
+  constexpr int S = kStride * 16;
+  if (left >= kBatch) {
+    copy16<0, 0>(dst, src);
+    copy16<S, S>(dst, src);
+    copy16<2 * S, 2 * S>(dst, src);
+    copy16<3 * S, 3 * S>(dst, src);
+  } else {
+    if (left > 0) copy16<0, 0>(dst, src); else sts128<0>(dst, neg_inf_vec<T>());
+    if (left > 1) copy16<S, S>(dst, src); else sts128<S>(dst, neg_inf_vec<T>());
+    if (left > 2) copy16<2 * S, 2 * S>(dst, src); else sts128<2 * S>(dst, neg_inf_vec<T>());
+    sts128<3 * S>(dst, neg_inf_vec<T>());
+  }
+}
+template <int kStride>
+__device__ __forceinline__ void read_batch(uint32_t src, uint4 (&r)[kBatch]) {
+  constexpr int S = kStride * 16;
+  r[0] = lds128<0>(src);
+  r[1] = lds128<S>(src);
+  r[2] = lds128<2 * S>(src);
+  r[3] = lds128<3 * S>(src);
+}
+template <int kStride>
+__device__ __forceinline__ void write_batch(uint32_t dst, const uint4 (&r)[kBatch]) {
+  constexpr int S = kStride * 16;
+  sts128<0>(dst, r[0]);
+  sts128<S>(dst, r[1]);
+  sts128<2 * S>(dst, r[2]);
+  sts128<3 * S>(dst, r[3]);
+}
+
 // One row of the launch. Whatever address it starts at, its entries are
 // `head` single ones up to a 16-byte boundary, nin full vectors, and a few
 // single ones behind; no access leaves the row.
@@ -261,29 +318,36 @@ template <typename T> struct Share {
   }
 };
 
+// Vectors of [begin, end) that this thread has when they go round the team.
+template <int kThreads> __device__ __forceinline__ int own_vectors(int begin, int end) {
+  return max(0, end - begin - Team<kThreads>::tid() + kThreads - 1) / kThreads;
+}
+
 // The vectors of a chunk pass through shared memory by asynchronous copies:
 // thread t copies, and alone reads, the vectors t, t + kThreads, ... of the
 // chunk, so it needs no barrier, all copies are in flight at once without a
-// register, and a row that fits is there for every later pass. Four groups,
-// so that the sums begin while most of the chunk is on its way.
+// register, and a row that fits is there for every later pass. They are asked
+// for in up to four groups, so that the sums begin while most is on its way.
 template <typename T, int kThreads>
 struct Stage {
-  uint4* buf;                      // this thread's first slot
-  int per;                         // vectors per group and thread
-  __device__ __forceinline__ Stage(uint4* chunk, int cap)
-      : buf(chunk + Team<kThreads>::tid()), per((cap / kThreads + 3) / 4) {}
-  // vectors of [base, end) that this thread has
-  __device__ __forceinline__ int count(int base, int end) const {
-    return max(0, end - base - Team<kThreads>::tid() + kThreads - 1) / kThreads;
-  }
+  uint32_t buf;                    // this thread's first slot
+  int per;                         // batches per group
+  __device__ __forceinline__ Stage(const void* chunk, int cap)
+      : buf(smem_u32(chunk) + Team<kThreads>::tid() * 16),
+        per((cap / (kBatch * kThreads) + 3) / 4) {}
   __device__ __forceinline__ void copy(const Row<T>& row, int base, int n) const {
-    const T* src = row.vec(base + Team<kThreads>::tid());
+    const char* src = reinterpret_cast<const char*>(row.vec(base + Team<kThreads>::tid()));
+    uint32_t dst = buf;
+    int left = n;
 #pragma unroll 1
     for (int q = 0; q < 4; ++q) {
-      const int e = min(n, (q + 1) * per);
-#pragma unroll 4
-      for (int i = q * per; i < e; ++i)
-        cp_async16(buf + i * kThreads, src + (long long)i * kThreads * Vec<T>::N, true);
+#pragma unroll 1
+      for (int b = 0; b < per && left > 0; ++b) {
+        copy_batch<T, kThreads>(dst, src, left);
+        dst += kBatch * kThreads * 16;
+        src += kBatch * kThreads * 16;
+        left -= kBatch;
+      }
       cp_async_commit();
     }
   }
@@ -314,9 +378,9 @@ __device__ __forceinline__ Sums single(float z, float c) {
   return {z, ex2((z - z) * c), 0.f};              // NaN for NaN and +inf
 }
 // Adds vectors, whose maximum is `top`, to the running sums: per entry one
-// exponential, half an add, a product and two sums each, and a clamp for the
-// entropy's 0 * -inf.
-template <typename T, int kVecs, bool kEntropy>
+// exponential and half an add, a product and a sum or two. With kClamp also a
+// clamp, for the entropy's 0 * -inf; without, t is NaN if there is a -inf.
+template <typename T, int kVecs, bool kEntropy, bool kClamp>
 __device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float top, float c, Sums& a) {
   constexpr int N = Vec<T>::N;
   if (top > a.m) {
@@ -339,11 +403,11 @@ __device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float top, f
       float2 x = __fmul2_rn(__fadd2_rn(float2{f[e], f[e + 1]}, nref), cc);
       const float2 p = {ex2(x.x), ex2(x.y)};
       s = __fadd2_rn(s, p);
-      if (kEntropy) {
+      if (kClamp) {
         x.x = fmaxf(x.x, -1000.f);
         x.y = fmaxf(x.y, -1000.f);
-        t = __ffma2_rn(p, x, t);
       }
+      if (kEntropy) t = __ffma2_rn(p, x, t);
     }
   }
   a.s += s.x + s.y;
@@ -391,30 +455,26 @@ __device__ __forceinline__ Sums team_sums(Sums a, float c, Sums* red) {
   return sum;
 }
 
-// A row that is read once goes through a ring of kBatches batches of four
-// vectors per thread: two batches are on their way while one is added up.
-constexpr int kBatch = 4, kBatches = 3, kSlots = kBatch * kBatches;
+// A row that is read once goes through a ring of two batches per thread: one
+// or two are on their way while one is added up.
+constexpr int kSlots = 2 * kBatch;
 
 template <typename T, int kThreads>
 struct Ring {
-  uint4* buf;                      // this thread's first slot
-  const T* src;                    // its next vector
+  uint32_t buf;                    // this thread's first slot
+  const char* src;                 // its next vector
   int left;                        // vectors not yet asked for
   int n;                           // vectors in all
-  __device__ __forceinline__ Ring(uint4* slots, const Row<T>& row, const Share<T>& share) {
-    buf = slots + Team<kThreads>::tid();
-    src = row.vec(share.begin + Team<kThreads>::tid());
-    n = left = max(0, share.end - share.begin - Team<kThreads>::tid() + kThreads - 1) / kThreads;
+  __device__ __forceinline__ Ring(const void* slots, const Row<T>& row, const Share<T>& share) {
+    buf = smem_u32(slots) + Team<kThreads>::tid() * 16;
+    src = reinterpret_cast<const char*>(row.vec(share.begin + Team<kThreads>::tid()));
+    n = left = own_vectors<kThreads>(share.begin, share.end);
   }
-  // asks for the next batch, into slots [slot, slot + 4); -inf behind the last vector
-  __device__ __forceinline__ void ask(int slot) {
+  // asks for the next batch into the half `at` of the ring
+  __device__ __forceinline__ void ask(uint32_t at) {
     if (left > 0) {
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (u < left) cp_async16(buf + (slot + u) * kThreads, src + u * kThreads * Vec<T>::N, true);
-        else buf[(slot + u) * kThreads] = neg_inf_vec<T>();
-      }
-      src += kBatch * kThreads * Vec<T>::N;
+      copy_batch<T, kThreads>(at, src, left);
+      src += kBatch * kThreads * 16;
       left -= kBatch;
     }
     cp_async_commit();
@@ -433,6 +493,8 @@ template <int kThreads> struct TopShared {
   static constexpr int kMaxCand = 512;
   unsigned long long cand[kMaxCand];
   uint32_t bound[Team<kThreads>::kWarps];
+  uint4 hold[Team<kThreads>::kWarps][32];
+  int hold_at[Team<kThreads>::kWarps][32];
   uint8_t list[Team<kThreads>::kWarps][32 * kBatch];
   int count;
   int red[Team<kThreads>::kWarps];
@@ -606,49 +668,66 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
     groups += __popc(vote);
   }
   __syncwarp();                                        // and the copies of the other lanes
-  auto push = [&](float z, int v) {
-    const int at = atomicAdd(&sh.count, 1);
-    if (at < TopShared<kThreads>::kMaxCand) sh.cand[at] = order_key(logit_key(z), v);
-  };
-  if (share.edge >= 0 && edge >= least) push(edge, share.edge);
   const int len = share.end - share.begin;
   const int per = (len + kBatch * kThreads - 1) / (kBatch * kThreads);   // vectors of a group
   const bool here = len <= kSlots * kThreads;          // the ring still holds the row
-  const int items = groups * per;
-  const uint4* slots = ring.buf - Tm::tid() + Tm::warp() * 32;
+  const uint32_t slots = ring.buf + (Tm::warp() * 32 - Tm::tid()) * 16;
+  uint4* hold = sh.hold[Tm::warp()];
+  int* hold_at = sh.hold_at[Tm::warp()];
+  // a group's vectors side by side on a power of two of lanes, as many groups as fit
+  const int lg = per > 16 ? 5 : per > 1 ? 32 - __clz(per - 1) : 0;
+  const int g_lane = Tm::lane() >> lg, g_step = 32 >> lg, i_lane = Tm::lane() & ((1 << lg) - 1);
+  const uint32_t before = (1u << Tm::lane()) - 1;
 #pragma unroll 1
-  for (int t0 = Tm::lane(); t0 < items; t0 += 32 * kBatch) {
-    uint4 r[kBatch];
-    int j[kBatch];
+  for (int g0 = 0; g0 < groups; g0 += kBatch * g_step) {
+#pragma unroll 1
+    for (int i0 = 0; i0 < per; i0 += 32) {
+      uint4 r[kBatch];
+      int j[kBatch];
 #pragma unroll
-    for (int x = 0; x < kBatch; ++x) {
-      const int t = t0 + 32 * x, g = t / per;
-      j[x] = -1;
-      r[x] = neg_inf_vec<T>();
-      if (t < items) {
-        const int who = list[g], i = (t - g * per) * kBatch + (who & (kBatch - 1));
+      for (int x = 0; x < kBatch; ++x) {
+        const int g = g0 + x * g_step + g_lane;
+        const int who = list[min(g, groups - 1)];
+        const int i = (i0 + i_lane) * kBatch + (who & (kBatch - 1));
         j[x] = share.begin + i * kThreads + Tm::warp() * 32 + who / kBatch;
-        if (j[x] < share.end)
-          r[x] = here ? slots[i * kThreads + who / kBatch]
-                      : __ldg(reinterpret_cast<const uint4*>(row.vec(j[x])));
+        if (g >= groups || i0 + i_lane >= per || j[x] >= share.end) j[x] = -1;
+        else if (here) r[x] = lds128<0>(slots + (i * kThreads + who / kBatch) * 16);
+        else r[x] = __ldg(reinterpret_cast<const uint4*>(row.vec(j[x])));
+      }
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        if (g0 + x * g_step >= groups) break;
+        if (kMask && !here && j[x] >= 0) row.apply_mask(r[x], j[x]);
+        const bool in = j[x] >= 0 && Vec<T>::max(r[x]) >= least;
+        const uint32_t vote = __ballot_sync(kAll, in);
+        if (!vote) continue;
+        // the vectors that reach the bound side by side, then one entry to a lane
+        if (in) {
+          hold[__popc(vote & before)] = r[x];
+          hold_at[__popc(vote & before)] = row.head + j[x] * N;
+        }
+        __syncwarp();
+        const int entries = __popc(vote) * N;
+#pragma unroll 1
+        for (int t0 = 0; t0 < entries; t0 += 32) {
+          const int t = t0 + Tm::lane();
+          float z = neg_inf();
+          if (t < entries) z = to_float(reinterpret_cast<const T*>(hold)[t]);
+          const bool top_z = z >= least;
+          const uint32_t hits = __ballot_sync(kAll, top_z);
+          int at = 0;
+          if (Tm::lane() == 0) at = atomicAdd(&sh.count, __popc(hits));
+          at = __shfl_sync(kAll, at, 0) + __popc(hits & before);
+          if (top_z && at < TopShared<kThreads>::kMaxCand)
+            sh.cand[at] = order_key(logit_key(z), hold_at[t / N] + (t & (N - 1)));
+        }
+        __syncwarp();
       }
     }
-#pragma unroll 1
-    for (int x = 0; x < kBatch; ++x) {
-      uint4 q = r[0];
-      if (x == 1) q = r[1];
-      if (x == 2) q = r[2];
-      if (x == 3) q = r[3];
-      const int jx = x == 0 ? j[0] : x == 1 ? j[1] : x == 2 ? j[2] : j[3];
-      if (jx < 0 || jx >= share.end) continue;
-      if (kMask && !here) row.apply_mask(q, jx);
-      if (!(Vec<T>::max(q) >= least)) continue;
-      float z[N];
-      Vec<T>::unpack(q, z);
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (z[e] >= least) push(z[e], row.head + jx * N + e);
-    }
+  }
+  if (share.edge >= 0 && edge >= least) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < TopShared<kThreads>::kMaxCand) sh.cand[at] = order_key(logit_key(edge), share.edge);
   }
   Tm::sync();
   const int n = sh.count;
@@ -696,31 +775,41 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
   const Row<T> row(a, r0);
   const Share<T> share(row, rank, log_blocks, Tm::tid());
   Ring<T, kThreads> ring(slots, row, share);
-  ring.ask(0);
-  ring.ask(kBatch);
+  uint32_t at = ring.buf;
+  constexpr uint32_t kHalf = kBatch * kThreads * 16;
+  ring.ask(at);
+  ring.ask(at + kHalf);
   float edge = neg_inf();
   if (share.edge >= 0) edge = row.at(share.edge);
+  // the first given entries are fetched while the row is on its way
+  long long given[2];
+  float given_z[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int k = Tm::tid() + q * kThreads;
+    given[q] = -1;
+    given_z[q] = 0.f;
+    if (rank == 0 && k < o.n_targets) given[q] = o.targets[row.index * o.n_targets + k];
+    if (given[q] >= 0 && given[q] < row.size) given_z[q] = row.at((int)given[q]);
+  }
   Sums sum = single(edge, a.c);
   float top[kBatch];
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) top[u] = neg_inf();
-  int slot = 0;
+  const bool keep = kMask && share.end - share.begin <= kSlots * kThreads;
+  bool clamp = kMask;                             // a warp that has met a -inf
 #pragma unroll 1
   for (int i = 0; i < ring.n; i += kBatch) {
-    cp_async_wait<kBatches - 2>();
+    cp_async_wait<1>();
     uint4 r[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) r[u] = ring.buf[(slot + u) * kThreads];
-    ring.ask(slot >= kBatch ? slot - kBatch : slot + (kBatches - 1) * kBatch);
+    read_batch<kThreads>(at, r);
     if (kMask) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (i + u < ring.n) {
+        if (i + u < ring.n)
           row.apply_mask(r[u], share.begin + (i + u) * kThreads + Tm::tid());
-          ring.buf[(slot + u) * kThreads] = r[u];
-        }
+      if (keep) write_batch<kThreads>(at, r);
     }
-    slot = slot == (kBatches - 1) * kBatch ? 0 : slot + kBatch;
     float all = neg_inf();
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -728,7 +817,19 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
       top[u] = fmaxf(top[u], t);
       all = fmaxf(all, t);
     }
-    accumulate<T, kBatch, true>(r, all, a.c, sum);
+    // `all` has every vector in it: they are in registers before their slots are filled again
+    asm volatile("" ::"f"(all) : "memory");
+    ring.ask(at);
+    at = at == ring.buf ? at + kHalf : ring.buf;
+    if (!clamp) {
+      const Sums before = sum;
+      accumulate<T, kBatch, true, false>(r, all, a.c, sum);
+      if (sum.t != sum.t) {
+        clamp = true;
+        sum = before;
+      }
+    } 
+    if (clamp) accumulate<T, kBatch, true, true>(r, all, a.c, sum);
   }
   cp_async_wait<0>();
   sum = team_sums<kThreads>(sum, a.c, sh.red);
@@ -767,15 +868,16 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
     }
   }
 #pragma unroll 1
-  for (int k = Tm::tid(); k < o.n_targets; k += kThreads) {
-    const long long i = o.targets[row.index * o.n_targets + k];
-    float lp = 0.f;
-    if (i >= row.size || bad) {
-      lp = i < 0 ? 0.f : quiet_nan();
-    } else if (i >= 0) {
-      const float z = row.at((int)i);
-      lp = z == neg_inf() ? z : (z - m) * a.inv_t - log_s;
+  for (int k = Tm::tid(), q = 0; k < o.n_targets; k += kThreads, ++q) {
+    long long i = q == 0 ? given[0] : given[1];
+    float z = q == 0 ? given_z[0] : given_z[1];
+    if (q > 1) {
+      i = o.targets[row.index * o.n_targets + k];
+      if (i >= 0 && i < row.size) z = row.at((int)i);
     }
+    float lp = z == neg_inf() ? z : (z - m) * a.inv_t - log_s;
+    if (bad || i >= row.size) lp = quiet_nan();
+    if (i < 0) lp = 0.f;
     o.log_probs[row.index * o.n_targets + k] = lp;
   }
   if (o.top_k == 0) return;
@@ -941,9 +1043,10 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
 // ------------------------------------------------------------ distillation
 // Shared memory of one team, in this order (dynamic): the chunk; p, logits,
 // indices of the list; and a bit per entry of the block's share (listed or
-// not), from 32 places before its first vector to 32 behind its last.
-__host__ __device__ constexpr int distill_bytes(int listed, int cap, int vecs, int n) {
-  return cap * 16 + (16 * listed + (vecs * n / 32 + 3) * 4 + 15) / 16 * 16;
+// not), from 32 places before its first vector to 32 behind its last chunk.
+__host__ __device__ constexpr int distill_bytes(int listed, int cap, int share, int n) {
+  return cap * 16 +
+         (16 * listed + ((share + cap - 1) / cap * cap * n / 32 + 3) * 4 + 15) / 16 * 16;
 }
 
 static __device__ __noinline__ double exp64(double x) { return exp(x); }
@@ -952,6 +1055,11 @@ static __device__ __noinline__ double exp64(double x) { return exp(x); }
 struct ListSums {
   double mass, p_log_p, p_z;       // sum P, P log P, P z' (relative to the largest z')
   float e;                         // sum exp(z')
+};
+// What every thread needs to know of the row for its gradient.
+struct DistillRow {
+  float coef, ref, nan;            // nan: 0, or NaN for a row without a distribution
+  float scale, big, norm, inv;     // of the listed entries
 };
 
 // The list's entries are dropped from the vectors before the one pass over
@@ -973,6 +1081,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   __shared__ ListSums lred[Tm::kPerBlock][Tm::kWarps];
   __shared__ float tops[Tm::kPerBlock][Tm::kWarps][2];
   __shared__ int flags[Tm::kPerBlock][Tm::kWarps];
+  __shared__ DistillRow done[Tm::kPerBlock];
   __shared__ float cl[kMaxCluster][2];            // every block's maximum and sum
   const int slot = Tm::slot(), K = o.n_listed;
   const int blocks = 1 << log_blocks, rank = blockIdx.x & (blocks - 1);
@@ -982,14 +1091,14 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   const Row<T> row(a, r0);
   const Share<T> share(row, rank, log_blocks, Tm::tid());
   unsigned char* mine = dyn + slot * team_bytes;
-  const Stage<T, kThreads> st(reinterpret_cast<uint4*>(mine), cap);
+  const Stage<T, kThreads> st(mine, cap);
   double* p = reinterpret_cast<double*>(mine + cap * 16);
   float* zu = reinterpret_cast<float*>(p + K);
   int* idx = reinterpret_cast<int*>(zu + K);
   uint32_t* bits = reinterpret_cast<uint32_t*>(idx + K);
   const bool one = share.end - share.begin <= cap, vec_store = row.vec_store();
   float weight = o.weight ? o.weight[row.index] : 1.f;
-  st.copy(row, share.begin, st.count(share.begin, min(share.begin + cap, share.end)));
+  st.copy(row, share.begin, own_vectors<kThreads>(share.begin, min(share.begin + cap, share.end)));
   if (weight == 0.f) {                            // nothing of the row is looked at
     cp_async_wait<0>();
     if (o.row_loss && rank == 0 && Tm::tid() == 0) o.row_loss[row.index] = 0.f;
@@ -1007,7 +1116,8 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   weight *= o.scale;
   if (o.upstream) weight *= o.upstream[row.index * o.upstream_stride];
   // entry v has the bit v - v0
-  const int v0 = row.head + share.begin * N - 32, words = (share.end - share.begin) * N / 32 + 3;
+  const int v0 = row.head + share.begin * N - 32;
+  const int words = (share.end - share.begin + cap - 1) / cap * cap * N / 32 + 3;
   for (int w = Tm::tid(); w < words; w += kThreads) bits[w] = 0u;
   bool bad = false, twice = false;
   float top_lp = neg_inf(), top_z = neg_inf();
@@ -1037,19 +1147,21 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       for (int q = 0; q < k; ++q) twice |= idx[q] == v;
     }
   }
+  const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
+  if (Tm::warp() < list_warps) {
 #pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    top_lp = fmaxf(top_lp, __shfl_xor_sync(0xffffffffu, top_lp, w));
-    top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
-  }
-  const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (twice ? 2u : 0u));
-  if (Tm::lane() == 0) {
-    tops[slot][Tm::warp()][0] = top_lp;
-    tops[slot][Tm::warp()][1] = top_z;
-    flags[slot][Tm::warp()] = flag;
+    for (int w = 16; w > 0; w >>= 1) {
+      top_lp = fmaxf(top_lp, __shfl_xor_sync(0xffffffffu, top_lp, w));
+      top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
+    }
+    const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (twice ? 2u : 0u));
+    if (Tm::lane() == 0) {
+      tops[slot][Tm::warp()][0] = top_lp;
+      tops[slot][Tm::warp()][1] = top_z;
+      flags[slot][Tm::warp()] = flag;
+    }
   }
   Tm::sync();
-  const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
   int all = 0;
   top_lp = top_z = neg_inf();
 #pragma unroll 1
@@ -1100,36 +1212,46 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   }
   // the rest of the row
   Sums sum{neg_inf(), 0.f, 0.f};
-  const int bit0 = Tm::tid() * N + 32;            // the thread's first bit in a chunk
+  constexpr int kStep = kThreads * N / 32;        // words of bits from one vector to the next
+  const uint32_t* my_bits = bits + 1 + (Tm::tid() * N >> 5);
+  const int my_shift = (Tm::tid() * N) & 31;
 #pragma unroll 1
   for (int base = share.begin; base < share.end; base += cap) {
-    const int n = st.count(base, min(base + cap, share.end));
+    const int n = own_vectors<kThreads>(base, min(base + cap, share.end));
     if (base != share.begin) st.copy(row, base, n);
+    const uint32_t* w = my_bits + (base - share.begin) * N / 32;
+    uint32_t at = st.buf;
+    int i = 0;
 #pragma unroll 1
     for (int q = 0; q < 4; ++q) {
       st.wait(q);
-      const int e = min(n, (q + 1) * st.per);
 #pragma unroll 1
-      for (int i = q * st.per; i < e; i += 2) {
-        uint4 r[2] = {st.buf[i * kThreads], neg_inf_vec<T>()};
-        if (i + 1 < e) r[1] = st.buf[(i + 1) * kThreads];
+      for (int b = 0; b < st.per && i < n; ++b, i += kBatch) {
+        uint4 r[kBatch];
+        read_batch<kThreads>(at, r);
         if (kMask) {
-          row.apply_mask(r[0], base + i * kThreads + Tm::tid());
-          st.buf[i * kThreads] = r[0];
-          if (i + 1 < e) {
-            row.apply_mask(r[1], base + (i + 1) * kThreads + Tm::tid());
-            st.buf[(i + 1) * kThreads] = r[1];
-          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u)
+            if (i + u < n) row.apply_mask(r[u], base + (i + u) * kThreads + Tm::tid());
+          write_batch<kThreads>(at, r);
         }
-        const int u = (base - share.begin + i * kThreads) * N + bit0;
-        const uint32_t b0 = (bits[u >> 5] >> (u & 31)) & ((1u << N) - 1u);
-        if (b0) drop_bits<T>(r[0], b0);
-        if (i + 1 < e) {
-          const int u1 = u + kThreads * N;
-          const uint32_t b1 = (bits[u1 >> 5] >> (u1 & 31)) & ((1u << N) - 1u);
-          if (b1) drop_bits<T>(r[1], b1);
+        constexpr uint32_t kOnes = (1u << N) - 1u;
+        uint32_t b4[kBatch], any = 0;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          b4[u] = w[u * kStep] >> my_shift;
+          any |= b4[u];
         }
-        accumulate<T, 2, false>(r, fmaxf(Vec<T>::max(r[0]), Vec<T>::max(r[1])), a.c, sum);
+        if (any & kOnes) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) drop_bits<T>(r[u], b4[u]);
+        }
+        w += kBatch * kStep;
+        at += kBatch * kThreads * 16;
+        float top = Vec<T>::max(r[0]);
+#pragma unroll
+        for (int u = 1; u < kBatch; ++u) top = fmaxf(top, Vec<T>::max(r[u]));
+        accumulate<T, kBatch, false, false>(r, top, a.c, sum);
       }
     }
   }
@@ -1149,71 +1271,91 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     }
     cluster_arrive();
     cluster_wait();
-    sum = {cl[0][0], cl[0][1], 0.f};
-#pragma unroll 1
-    for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
   }
-  ListSums ls{0.0, 0.0, 0.0, 0.f};
+  if (Tm::warp() == 0) {
+    // one warp for all: loss and coefficients
+    if (blocks > 1) {
+      sum = {cl[0][0], cl[0][1], 0.f};
 #pragma unroll 1
-  for (int w = 0; w < list_warps; ++w) {
-    ls.mass += lred[slot][w].mass;
-    ls.p_log_p += lred[slot][w].p_log_p;
-    ls.p_z += lred[slot][w].p_z;
-    ls.e += lred[slot][w].e;
-  }
-  const bool rest = sum.m != neg_inf(), listed = top_z != neg_inf();
-  bad |= sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
-  const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
-  const double inv = whole && ls.mass > 0.0 ? 1.0 / ls.mass : 1.0;
-  const float p_r = whole ? 0.f : (float)(1.0 - ls.mass);
-  const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
-  // the two normalisers relative to the larger of the two maxima
-  const float big = fmaxf(rest ? sum.m : neg_inf(), top_z);
-  const float down_r = rest ? (sum.m - big) * a.inv_t : 0.f;
-  const float down_u = listed ? (top_z - big) * a.inv_t : 0.f;
-  const float norm_r = rest ? sum.s * expf(down_r) : 0.f;
-  const float norm = norm_r + (listed ? ls.e * expf(down_u) : 0.f);
-  const float log_all = logf(norm);
-  if (rank == 0 && Tm::tid() == 0 && o.row_loss) {
-    double loss = 0.0;
-    if (live && ls.mass > 0.0)
-      loss = inv * (ls.p_log_p - ls.p_z + ((double)log_all - (double)down_u) * ls.mass) +
-             (whole ? log(inv) * (inv * ls.mass) : 0.0);
-    if (live && p_r > 0.f)
-      loss += (double)p_r * ((double)logf(p_r) -
-                             ((double)down_r + (double)logf(sum.s) - (double)log_all));
-    o.row_loss[row.index] =
-        bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
+      for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
+    }
+    ListSums ls{0.0, 0.0, 0.0, 0.f};
+#pragma unroll 1
+    for (int w = 0; w < list_warps; ++w) {
+      ls.mass += lred[slot][w].mass;
+      ls.p_log_p += lred[slot][w].p_log_p;
+      ls.p_z += lred[slot][w].p_z;
+      ls.e += lred[slot][w].e;
+    }
+    const bool rest = sum.m != neg_inf(), listed = top_z != neg_inf();
+    bad |= sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
+    const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
+    const double inv = whole && ls.mass > 0.0 ? 1.0 / ls.mass : 1.0;
+    const float p_r = whole ? 0.f : (float)(1.0 - ls.mass);
+    const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
+    // the two normalisers relative to the larger of the two maxima
+    const float big = fmaxf(rest ? sum.m : neg_inf(), top_z);
+    const float down_r = rest ? (sum.m - big) * a.inv_t : 0.f;
+    const float down_u = listed ? (top_z - big) * a.inv_t : 0.f;
+    const float norm_r = rest ? sum.s * expf(down_r) : 0.f;
+    const float norm = norm_r + (listed ? ls.e * expf(down_u) : 0.f);
+    if (rank == 0 && Tm::tid() == 0 && o.row_loss) {
+      const float log_all = logf(norm);
+      double loss = 0.0;
+      if (live && ls.mass > 0.0)
+        loss = inv * (ls.p_log_p - ls.p_z + ((double)log_all - (double)down_u) * ls.mass) +
+               (whole ? log(inv) * (inv * ls.mass) : 0.0);
+      if (live && p_r > 0.f)
+        loss += (double)p_r * ((double)logf(p_r) -
+                               ((double)down_r + (double)logf(sum.s) - (double)log_all));
+      o.row_loss[row.index] =
+          bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
+    }
+    if (Tm::tid() == 0) {
+      const float scale = live ? weight * a.t : 0.f;
+      const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
+      done[slot] = {coef, rest ? sum.m : 0.f, bad || coef != coef ? quiet_nan() : 0.f,
+                    scale, big, norm, (float)inv};
+    }
   }
   if (!row.grad) return;
-  const float scale = weight * a.t;
-  const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
-  const float ref = rest ? sum.m : 0.f, nan = quiet_nan();
-  bad |= coef != coef;
-  const float2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
-  if (!bad) {
+  Tm::sync();
+  const DistillRow d = done[slot];
+  const float2 nref = {-d.ref, -d.ref}, cc = {a.c, a.c}, kk = {d.coef, d.coef};
+  auto slope = [&](const uint4& r, int j) {
+    float z[N];
+    Vec<T>::unpack(r, z);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float2 x = __fmul2_rn(__fadd2_rn(float2{z[e], z[e + 1]}, nref), cc);
+      const float2 g = __fmul2_rn(float2{ex2(x.x), ex2(x.y)}, kk);
+      z[e] = g.x;
+      z[e + 1] = g.y;
+    }
+    row.store(j, z, vec_store);
+  };
+  if (d.nan == 0.f) {
 #pragma unroll 1
     for (int base = share.begin; base < share.end; base += cap) {
-      const int n = st.count(base, min(base + cap, share.end));
+      const int n = own_vectors<kThreads>(base, min(base + cap, share.end));
       if (!one) {
         st.copy(row, base, n);
         cp_async_wait<0>();
       }
-#pragma unroll 2
-      for (int i = 0; i < n; ++i) {
-        const int j = base + i * kThreads + Tm::tid();
-        uint4 r = st.buf[i * kThreads];
-        if (kMask && !one) row.apply_mask(r, j);
-        float z[N];
-        Vec<T>::unpack(r, z);
+      uint32_t at = st.buf;
+      int j = base + Tm::tid();
+#pragma unroll 1
+      for (int i = 0; i < n; i += kBatch) {
+        uint4 r[kBatch];
+        read_batch<kThreads>(at, r);
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const float2 x = __fmul2_rn(__fadd2_rn(float2{z[e], z[e + 1]}, nref), cc);
-          const float2 d = __fmul2_rn(float2{ex2(x.x), ex2(x.y)}, kk);
-          z[e] = d.x;
-          z[e + 1] = d.y;
+        for (int u = 0; u < kBatch; ++u) {
+          if (i + u >= n) break;
+          if (kMask && !one) row.apply_mask(r[u], j + u * kThreads);
+          slope(r[u], j + u * kThreads);
         }
-        row.store(j, z, vec_store);
+        at += kBatch * kThreads * 16;
+        j += kBatch * kThreads;
       }
     }
   } else {
@@ -1221,16 +1363,15 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   }
   if (share.edge >= 0)
     row.grad[share.edge] =
-        to_type<T>(edge == neg_inf() ? 0.f : bad ? nan : ex2((edge - ref) * a.c) * coef);
+        to_type<T>(edge == neg_inf() ? 0.f : d.nan + ex2((edge - d.ref) * a.c) * d.coef);
   if (K == 0) return;
   Tm::sync();                                     // the listed entries are written again
 #pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
     const int v = idx[k];
     if (v < share.first || v >= share.last) continue;
-    const float q = expf((zu[k] - big) * a.inv_t) / norm;
-    const float d = live ? scale * (q - (float)(p[k] * inv)) : 0.f;
-    row.grad[v] = to_type<T>(bad ? nan : d);
+    const float q = expf((zu[k] - d.big) * a.inv_t) / d.norm;
+    row.grad[v] = to_type<T>(d.nan + d.scale * (q - (float)p[k] * d.inv));
   }
 }
 

@@ -13,7 +13,7 @@ namespace lk {
 namespace {
 
 // How a launch is cut: threads of a team, blocks of a row's cluster (a power
-// of two), and the vectors of a block's chunk (a multiple of the threads).
+// of two), and the vectors of a block's chunk (a multiple of kBatch times the threads).
 struct Cut {
   int threads, log_blocks, cap;
 };
@@ -33,7 +33,7 @@ Cut cut_rows(int nvec, long long rows, bool warp) {
   c.threads = warp && share <= 64 ? 32 : share <= 1024 ? 128 : share <= 4096 ? 256 : 512;
   if (c.log_blocks && c.threads < 256) c.threads = 256;
   const int most = std::min(std::max(share, 1), kChunkBytes / 16);
-  c.cap = (most + c.threads - 1) / c.threads * c.threads;
+  c.cap = (most + kBatch * c.threads - 1) / (kBatch * c.threads) * (kBatch * c.threads);
   return c;
 }
 
