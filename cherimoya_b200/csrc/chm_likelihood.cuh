@@ -53,6 +53,12 @@ template <> struct Vec<float> {
     return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
                  fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
+  // running maxima of one or more vectors, kept in the type's own width
+  using Max = float;
+  static __device__ __forceinline__ Max lowest() { return __uint_as_float(kNegInf); }
+  static __device__ __forceinline__ Max wide_max(const uint4& r) { return max(r); }
+  static __device__ __forceinline__ Max larger(Max a, Max b) { return fmaxf(a, b); }
+  static __device__ __forceinline__ float to_max(Max a) { return a; }
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
@@ -74,11 +80,21 @@ template <> struct Vec<__nv_bfloat16> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+  // running maxima of one or more vectors, kept in pairs of the type's own width
+  using Max = __nv_bfloat162;
+  static __device__ __forceinline__ Max lowest() {
+    const uint32_t v = kNegInf;
+    return reinterpret_cast<const Max&>(v);
   }
+  static __device__ __forceinline__ Max wide_max(const uint4& r) {
+    const Max* h = reinterpret_cast<const Max*>(&r);
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  }
+  static __device__ __forceinline__ Max larger(Max a, Max b) { return __hmax2(a, b); }
+  static __device__ __forceinline__ float to_max(Max a) {
+    return fmaxf(__low2float(a), __high2float(a));
+  }
+  static __device__ __forceinline__ float max(const uint4& r) { return to_max(wide_max(r)); }
 };
 template <> struct Vec<__half> {
   static constexpr int N = 8;
@@ -101,11 +117,21 @@ template <> struct Vec<__half> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    const __half2* h = reinterpret_cast<const __half2*>(&r);
-    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+  // running maxima of one or more vectors, kept in pairs of the type's own width
+  using Max = __half2;
+  static __device__ __forceinline__ Max lowest() {
+    const uint32_t v = kNegInf;
+    return reinterpret_cast<const Max&>(v);
   }
+  static __device__ __forceinline__ Max wide_max(const uint4& r) {
+    const Max* h = reinterpret_cast<const Max*>(&r);
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  }
+  static __device__ __forceinline__ Max larger(Max a, Max b) { return __hmax2(a, b); }
+  static __device__ __forceinline__ float to_max(Max a) {
+    return fmaxf(__low2float(a), __high2float(a));
+  }
+  static __device__ __forceinline__ float max(const uint4& r) { return to_max(wide_max(r)); }
 };
 
 // Writes -inf over element E of a vector.
@@ -598,9 +624,10 @@ __device__ __noinline__ int thin_out(int n, int k, TopShared<kThreads>& sh) {
 // While the row passes, each thread keeps four maxima, one for every fourth of
 // its vectors: 4 * kThreads groups in all. If k of the groups have a maximum
 // of at least b, then k entries do, so every entry at or above b is a
-// candidate and only those groups are looked at again. b comes from bisection
-// over the maxima: in each warp for the ceil(k / warps)-th, and where the
-// warps differ too much (a profile's summit lies in few of them) over all.
+// candidate and only those groups are looked at again. b is the smallest over
+// the warps of the ceil(k / warps)-th largest maximum of each, and where the
+// warps differ too much (a profile's summit lies in few of them) it comes from
+// bisection over all.
 template <typename T, int kThreads, bool kMask>
 __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& share,
                                            const Ring<T, kThreads>& ring, float edge,
@@ -622,17 +649,44 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
     return n;
   };
   const int want = (k + Tm::kWarps - 1) / Tm::kWarps;
-  // 32 maxima reach the smallest of the lanes' largest
-  uint32_t lo = want <= 32 ? __reduce_min_sync(kAll, most) : 0u;
-  uint32_t hi = __reduce_max_sync(kAll, most) + 1;
-  for (int n = 128; hi - lo > 1 && n > want + want / 4;) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    const int r = __reduce_add_sync(kAll, reach(mid));
-    if (r >= want) {
-      lo = mid;
-      n = r;
-    } else {
-      hi = mid;
+  uint32_t lo = 0;
+  if (want <= 12) {
+    // the want-th largest, one by one: each lane's maxima sorted, its largest first
+    uint32_t q[kBatch] = {key[0], key[1], key[2], key[3]};
+    auto order = [](uint32_t& x, uint32_t& y) {
+      const uint32_t t = max(x, y);
+      y = min(x, y);
+      x = t;
+    };
+    order(q[0], q[1]);
+    order(q[2], q[3]);
+    order(q[0], q[2]);
+    order(q[1], q[3]);
+    order(q[1], q[2]);
+#pragma unroll 1
+    for (int i = 0; i < want; ++i) {
+      lo = __reduce_max_sync(kAll, q[0]);
+      const uint32_t vote = __ballot_sync(kAll, q[0] == lo);
+      if (Tm::lane() == __ffs(vote) - 1) {
+        q[0] = q[1];
+        q[1] = q[2];
+        q[2] = q[3];
+        q[3] = 0;
+      }
+    }
+  } else {
+    // 32 maxima reach the smallest of the lanes' largest
+    if (want <= 32) lo = __reduce_min_sync(kAll, most);
+    uint32_t hi = __reduce_max_sync(kAll, most) + 1;
+    for (int n = 128; hi - lo > 1 && n > want + want / 4;) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int r = __reduce_add_sync(kAll, reach(mid));
+      if (r >= want) {
+        lo = mid;
+        n = r;
+      } else {
+        hi = mid;
+      }
     }
   }
   if (Tm::tid() == 0) sh.count = 0;
@@ -793,9 +847,9 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
     if (given[q] >= 0 && given[q] < row.size) given_z[q] = row.at((int)given[q]);
   }
   Sums sum = single(edge, a.c);
-  float top[kBatch];
+  typename Vec<T>::Max tops[kBatch];
 #pragma unroll
-  for (int u = 0; u < kBatch; ++u) top[u] = neg_inf();
+  for (int u = 0; u < kBatch; ++u) tops[u] = Vec<T>::lowest();
   const bool keep = kMask && share.end - share.begin <= kSlots * kThreads;
   bool clamp = kMask;                             // a warp that has met a -inf
 #pragma unroll 1
@@ -810,13 +864,15 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
           row.apply_mask(r[u], share.begin + (i + u) * kThreads + Tm::tid());
       if (keep) write_batch<kThreads>(at, r);
     }
-    float all = neg_inf();
+    typename Vec<T>::Max most = Vec<T>::wide_max(r[0]);
+    tops[0] = Vec<T>::larger(tops[0], most);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const float t = Vec<T>::max(r[u]);
-      top[u] = fmaxf(top[u], t);
-      all = fmaxf(all, t);
+    for (int u = 1; u < kBatch; ++u) {
+      const typename Vec<T>::Max t = Vec<T>::wide_max(r[u]);
+      tops[u] = Vec<T>::larger(tops[u], t);
+      most = Vec<T>::larger(most, t);
     }
+    const float all = Vec<T>::to_max(most);
     // `all` has every vector in it: they are in registers before their slots are filled again
     asm volatile("" ::"f"(all) : "memory");
     ring.ask(at);
@@ -834,7 +890,12 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
   cp_async_wait<0>();
   sum = team_sums<kThreads>(sum, a.c, sh.red);
   int n = 0;
-  if (o.top_k > 0) n = collect_top<T, kThreads, kMask>(row, share, ring, edge, top, o.top_k, sh.top);
+  if (o.top_k > 0) {
+    float top[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) top[u] = Vec<T>::to_max(tops[u]);
+    n = collect_top<T, kThreads, kMask>(row, share, ring, edge, top, o.top_k, sh.top);
+  }
   const unsigned long long* keys = sh.top.cand;
   if (blocks > 1) {
     // the share's sums and its sorted top entries go to the first block
@@ -1248,10 +1309,10 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
         }
         w += kBatch * kStep;
         at += kBatch * kThreads * 16;
-        float top = Vec<T>::max(r[0]);
+        typename Vec<T>::Max most = Vec<T>::wide_max(r[0]);
 #pragma unroll
-        for (int u = 1; u < kBatch; ++u) top = fmaxf(top, Vec<T>::max(r[u]));
-        accumulate<T, kBatch, false, false>(r, top, a.c, sum);
+        for (int u = 1; u < kBatch; ++u) most = Vec<T>::larger(most, Vec<T>::wide_max(r[u]));
+        accumulate<T, kBatch, false, false>(r, Vec<T>::to_max(most), a.c, sum);
       }
     }
   }
