@@ -134,26 +134,6 @@ template <> struct Vec<__half> {
   static __device__ __forceinline__ float max(const uint4& r) { return to_max(wide_max(r)); }
 };
 
-// Writes -inf over element E of a vector.
-template <typename T, int E> __device__ __forceinline__ void drop(uint4& r) {
-  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-  if constexpr (sizeof(T) == 4) {
-    w[E] = Vec<T>::kNegInf;
-  } else if constexpr (E % 2 == 0) {
-    w[E / 2] = (w[E / 2] & 0xffff0000u) | (Vec<T>::kNegInf & 0xffffu);
-  } else {
-    w[E / 2] = (w[E / 2] & 0xffffu) | (Vec<T>::kNegInf & 0xffff0000u);
-  }
-}
-// -inf over the elements whose bit is set
-template <typename T, int E = 0> __device__ __forceinline__ void drop_bits(uint4& r, uint32_t b) {
-  if constexpr (E < Vec<T>::N) {
-    if ((b >> E) & 1u) drop<T, E>(r);
-    drop_bits<T, E + 1>(r, b);
-  }
-}
-
-// -inf over element e of a vector in shared memory order
 template <typename T>
 __device__ __forceinline__ uint4 neg_inf_vec() {
   return make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
@@ -216,6 +196,14 @@ __device__ __forceinline__ void write_batch(uint32_t dst, const uint4 (&r)[kBatc
   sts128<3 * S>(dst, r[3]);
 }
 
+// Each byte of the result is 0xff or 0: the top bit of the byte of t that the
+// selector's digit (less 8) names.
+template <uint32_t kSel> __device__ __forceinline__ uint32_t spread(uint32_t t) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(r) : "r"(t), "n"(kSel));
+  return r;
+}
+
 // One row of the launch. Whatever address it starts at, its entries are
 // `head` single ones up to a 16-byte boundary, nin full vectors, and a few
 // single ones behind; no access leaves the row.
@@ -247,22 +235,44 @@ struct Row {
     return (mask && !mask[v]) ? neg_inf() : to_float(z[v]);
   }
   __device__ __forceinline__ const T* vec(int j) const { return z + head + (long long)j * N; }
-  // vector j with -inf over what the mask takes out
-  __device__ __forceinline__ void apply_mask(uint4& r, int j) const {
+  // the mask's bytes for vector j
+  struct MaskBytes {
+    uint32_t w[N / 4];
+  };
+  __device__ __forceinline__ MaskBytes mask_bytes(int j) const {
     const uint8_t* m = mask + head + (long long)j * N;
-    uint32_t b = 0;
+    MaskBytes b;
     if ((reinterpret_cast<uintptr_t>(m) & (N - 1)) == 0) {
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(m)[i];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b |= ((w >> (8 * e)) & 0xffu) ? 0u : 1u << (4 * i + e);
-      }
+      for (int i = 0; i < N / 4; ++i) b.w[i] = reinterpret_cast<const uint32_t*>(m)[i];
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) b |= m[e] ? 0u : 1u << e;
+      for (int i = 0; i < N / 4; ++i)
+        b.w[i] = m[4 * i] | m[4 * i + 1] << 8 | m[4 * i + 2] << 16 | (uint32_t)m[4 * i + 3] << 24;
     }
-    if (b) drop_bits<T>(r, b);
+    return b;
+  }
+  // -inf over what the mask takes out
+  static __device__ __forceinline__ void apply_mask(uint4& r, const MaskBytes& b) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      // the top bit of every byte that is not zero
+      const uint32_t t = ((b.w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | b.w[i];
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t on[4] = {spread<0x8888>(t), spread<0x9999>(t), spread<0xaaaa>(t),
+                                spread<0xbbbb>(t)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (v[e] & on[e]) | (Vec<T>::kNegInf & ~on[e]);
+      } else {
+        const uint32_t on0 = spread<0x9988>(t), on1 = spread<0xbbaa>(t);
+        v[2 * i] = (v[2 * i] & on0) | (Vec<T>::kNegInf & ~on0);
+        v[2 * i + 1] = (v[2 * i + 1] & on1) | (Vec<T>::kNegInf & ~on1);
+      }
+    }
+  }
+  __device__ __forceinline__ void apply_mask(uint4& r, int j) const {
+    apply_mask(r, mask_bytes(j));
   }
   __device__ __forceinline__ void store(int j, const float (&d)[N], bool vec_store) const {
     T* g = grad + head + (long long)j * N;
@@ -350,42 +360,21 @@ template <int kThreads> __device__ __forceinline__ int own_vectors(int begin, in
 }
 
 // The vectors of a chunk pass through shared memory by asynchronous copies:
-// thread t copies, and alone reads, the vectors t, t + kThreads, ... of the
-// chunk, so it needs no barrier, all copies are in flight at once without a
-// register, and a row that fits is there for every later pass. They are asked
-// for in up to four groups, so that the sums begin while most is on its way.
+// thread t copies, and sums up, the vectors t, t + kThreads, ... of the chunk.
+// All of them are in flight at once without a register, and a row that fits
+// is there for every later pass. In shared memory the chunk is as in memory.
 template <typename T, int kThreads>
-struct Stage {
-  uint32_t buf;                    // this thread's first slot
-  int per;                         // batches per group
-  __device__ __forceinline__ Stage(const void* chunk, int cap)
-      : buf(smem_u32(chunk) + Team<kThreads>::tid() * 16),
-        per((cap / (kBatch * kThreads) + 3) / 4) {}
-  __device__ __forceinline__ void copy(const Row<T>& row, int base, int n) const {
-    const char* src = reinterpret_cast<const char*>(row.vec(base + Team<kThreads>::tid()));
-    uint32_t dst = buf;
-    int left = n;
+__device__ __forceinline__ void copy_chunk(uint32_t chunk, const Row<T>& row, int base, int n) {
+  const char* src = reinterpret_cast<const char*>(row.vec(base + Team<kThreads>::tid()));
+  uint32_t dst = chunk + Team<kThreads>::tid() * 16;
 #pragma unroll 1
-    for (int q = 0; q < 4; ++q) {
-#pragma unroll 1
-      for (int b = 0; b < per && left > 0; ++b) {
-        copy_batch<T, kThreads>(dst, src, left);
-        dst += kBatch * kThreads * 16;
-        src += kBatch * kThreads * 16;
-        left -= kBatch;
-      }
-      cp_async_commit();
-    }
+  for (; n > 0; n -= kBatch) {
+    copy_batch<T, kThreads>(dst, src, n);
+    dst += kBatch * kThreads * 16;
+    src += kBatch * kThreads * 16;
   }
-  __device__ __forceinline__ void wait(int q) const {
-    switch (q) {
-      case 0: cp_async_wait<3>(); break;
-      case 1: cp_async_wait<2>(); break;
-      case 2: cp_async_wait<1>(); break;
-      default: cp_async_wait<0>();
-    }
-  }
-};
+  cp_async_commit();
+}
 
 // Running maximum m, s = sum 2^x and t = sum x 2^x with x = (z - m) c.
 struct Sums {
@@ -851,7 +840,15 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) tops[u] = Vec<T>::lowest();
   const bool keep = kMask && share.end - share.begin <= kSlots * kThreads;
-  bool clamp = kMask;                             // a warp that has met a -inf
+  bool clamp = kMask;                             // this thread has met a -inf
+  typename Row<T>::MaskBytes ahead[kBatch];       // of the next batch
+  auto fetch_mask = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (i + u < ring.n)
+        ahead[u] = row.mask_bytes(share.begin + (i + u) * kThreads + Tm::tid());
+  };
+  if (kMask) fetch_mask(0);
 #pragma unroll 1
   for (int i = 0; i < ring.n; i += kBatch) {
     cp_async_wait<1>();
@@ -860,8 +857,8 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
     if (kMask) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (i + u < ring.n)
-          row.apply_mask(r[u], share.begin + (i + u) * kThreads + Tm::tid());
+        if (i + u < ring.n) Row<T>::apply_mask(r[u], ahead[u]);
+      fetch_mask(i + kBatch);
       if (keep) write_batch<kThreads>(at, r);
     }
     typename Vec<T>::Max most = Vec<T>::wide_max(r[0]);
@@ -1102,45 +1099,92 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
 }
 
 // ------------------------------------------------------------ distillation
-// Shared memory of one team, in this order (dynamic): the chunk; p, logits,
-// indices of the list; and a bit per entry of the block's share (listed or
-// not), from 32 places before its first vector to 32 behind its last chunk.
-__host__ __device__ constexpr int distill_bytes(int listed, int cap, int share, int n) {
-  return cap * 16 +
-         (16 * listed + ((share + cap - 1) / cap * cap * n / 32 + 3) * 4 + 15) / 16 * 16;
+// Shared memory of one team, in this order (dynamic): one or two chunks; p,
+// logits, indices of the list; a bit per entry of the row (modulo kSeenBits).
+constexpr int kSeenBits = 1 << 15;
+__host__ __device__ constexpr int seen_words(int size) {
+  return ((size < kSeenBits ? size : kSeenBits) + 31) / 32;
+}
+__host__ __device__ constexpr int distill_bytes(int listed, int cap, int chunks, int largest) {
+  return chunks * cap * 16 + 16 * listed + (seen_words(largest) * 4 + 15) / 16 * 16;
+}
+
+template <typename T> __device__ __forceinline__ void sts_neg_inf(uint32_t a) {
+  if constexpr (sizeof(T) == 4)
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(Vec<T>::kNegInf) : "memory");
+  else
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((uint16_t)Vec<T>::kNegInf) : "memory");
 }
 
 static __device__ __noinline__ double exp64(double x) { return exp(x); }
 
 // Per warp: what the list adds up to.
 struct ListSums {
-  double mass, p_log_p, p_z;       // sum P, P log P, P z' (relative to the largest z')
+  double mass, p_log_p, p_z;       // sum P, P log P, P z'
   float e;                         // sum exp(z')
+  float top_z, top_lp;             // the warp's largest z, log P: z' and P are relative to them
 };
+// A list in which an entry may be twice: the first one takes the others' mass
+// (p: log P before and after), the others leave the list. Marks can coincide
+// without a repeat, so most calls find none.
+template <int kThreads>
+__device__ __noinline__ void merge_list(double* p, int* idx, int K) {
+  using Tm = Team<kThreads>;
+  uint32_t gone = 0;                              // of this thread's entries, in order
+#pragma unroll 1
+  for (int k = Tm::tid(), i = 0; k < K; k += kThreads, ++i) {
+    const int v = idx[k];
+    if (v < 0) continue;
+    bool first = true;
+    for (int q = 0; q < k && first; ++q) first = idx[q] != v;
+    if (!first) {
+      gone |= 1u << i;
+      continue;
+    }
+    double top = p[k];
+    for (int q = k + 1; q < K; ++q)
+      if (idx[q] == v) top = fmax(top, p[q]);
+    double mass = exp64(p[k] - top);
+    bool alone = true;
+    for (int q = k + 1; q < K; ++q)
+      if (idx[q] == v) {
+        mass += exp64(p[q] - top);
+        alone = false;
+      }
+    if (!alone && top > (double)neg_inf()) p[k] = top + log(mass);
+  }
+  Tm::sync();
+#pragma unroll 1
+  for (int k = Tm::tid(), i = 0; k < K; k += kThreads, ++i)
+    if ((gone >> i) & 1u) idx[k] = -1;
+  Tm::sync();
+}
+
 // What every thread needs to know of the row for its gradient.
 struct DistillRow {
   float coef, ref, nan;            // nan: 0, or NaN for a row without a distribution
   float scale, big, norm, inv;     // of the listed entries
 };
 
-// The list's entries are dropped from the vectors before the one pass over
-// the row, so that pass gives maximum and sum over the rest alone, without a
-// difference of nearly equal numbers; the teacher's masses are added in 64
-// bits, for the rest's is 1 minus their sum. With lse_R, lse the logs of the
-// two normalisers and q_R = exp(lse_R - lse)
+// The list's entries are overwritten by -inf in shared memory before the one
+// pass over the row, so that pass gives maximum and sum over the rest alone,
+// without a difference of nearly equal numbers; the teacher's masses are added
+// in 64 bits, for the rest's is 1 minus their sum. With lse_R, lse the logs of
+// the two normalisers and q_R = exp(lse_R - lse)
 //   dz_v = T w exp(z'_v - lse_R) (q_R - P_rest)     outside the list
 //   dz_u = T w (exp(z'_u - lse) - P_u)              in it
-// so the gradient is one more exponential per entry in shared memory.
+// so the gradient is one more exponential per entry in shared memory. Without
+// a gradient the chunks are small and there are two, one on its way.
 template <typename T, int kThreads, bool kMask>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock)
 distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned rows, int log_blocks,
-               int cap, int team_bytes) {
+               int cap, int chunks, int team_bytes) {
   using Tm = Team<kThreads>;
   constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Sums red[Tm::kPerBlock][Tm::kWarps];
   __shared__ ListSums lred[Tm::kPerBlock][Tm::kWarps];
-  __shared__ float tops[Tm::kPerBlock][Tm::kWarps][2];
+  __shared__ float factor[Tm::kPerBlock][Tm::kWarps];   // of a warp's p, to that of all
   __shared__ int flags[Tm::kPerBlock][Tm::kWarps];
   __shared__ DistillRow done[Tm::kPerBlock];
   __shared__ float cl[kMaxCluster][2];            // every block's maximum and sum
@@ -1152,14 +1196,15 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   const Row<T> row(a, r0);
   const Share<T> share(row, rank, log_blocks, Tm::tid());
   unsigned char* mine = dyn + slot * team_bytes;
-  const Stage<T, kThreads> st(mine, cap);
-  double* p = reinterpret_cast<double*>(mine + cap * 16);
+  const uint32_t chunk = smem_u32(mine);
+  double* p = reinterpret_cast<double*>(mine + chunks * cap * 16);
   float* zu = reinterpret_cast<float*>(p + K);
   int* idx = reinterpret_cast<int*>(zu + K);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(idx + K);
+  uint32_t* seen = reinterpret_cast<uint32_t*>(idx + K);
   const bool one = share.end - share.begin <= cap, vec_store = row.vec_store();
   float weight = o.weight ? o.weight[row.index] : 1.f;
-  st.copy(row, share.begin, own_vectors<kThreads>(share.begin, min(share.begin + cap, share.end)));
+  copy_chunk<T, kThreads>(chunk, row, share.begin,
+                          own_vectors<kThreads>(share.begin, min(share.begin + cap, share.end)));
   if (weight == 0.f) {                            // nothing of the row is looked at
     cp_async_wait<0>();
     if (o.row_loss && rank == 0 && Tm::tid() == 0) o.row_loss[row.index] = 0.f;
@@ -1176,12 +1221,9 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   }
   weight *= o.scale;
   if (o.upstream) weight *= o.upstream[row.index * o.upstream_stride];
-  // entry v has the bit v - v0
-  const int v0 = row.head + share.begin * N - 32;
-  const int words = (share.end - share.begin + cap - 1) / cap * cap * N / 32 + 3;
-  for (int w = Tm::tid(); w < words; w += kThreads) bits[w] = 0u;
-  bool bad = false, twice = false;
-  float top_lp = neg_inf(), top_z = neg_inf();
+  const int words = seen_words(row.size);
+  for (int w = Tm::tid(); w < words; w += kThreads) seen[w] = 0u;
+  bool bad = false;
 #pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
     const long long i = o.indices[row.index * K + k];
@@ -1192,67 +1234,45 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     idx[k] = there ? (int)i : -1;
     zu[k] = z;
     p[k] = (double)lp;
-    if (there) {
-      top_lp = fmaxf(top_lp, lp);
-      top_z = fmaxf(top_z, z);
-    }
-  }
-  Tm::sync();
-#pragma unroll 1
-  for (int k = Tm::tid(); k < K; k += kThreads) {
-    const int v = idx[k];
-    if (v >= share.first && v < share.last) {
-      const uint32_t old = atomicOr(&bits[(v - v0) >> 5], 1u << ((v - v0) & 31));
-      twice |= (old >> ((v - v0) & 31)) & 1u;
-    } else if (v >= 0) {                          // repeats in the other blocks' shares
-      for (int q = 0; q < k; ++q) twice |= idx[q] == v;
-    }
   }
   const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
-  if (Tm::warp() < list_warps) {
+  // marks the list's entries, to see whether one is there twice
+  auto mark = [&]() {
+    if (Tm::warp() >= list_warps) return;
+    bool again = false;
+#pragma unroll 1
+    for (int k = Tm::tid(); k < K; k += kThreads) {
+      const int v = idx[k] & (kSeenBits - 1);
+      if (idx[k] >= 0) again |= (atomicOr(&seen[v >> 5], 1u << (v & 31)) >> (v & 31)) & 1u;
+    }
+    const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (again ? 2u : 0u));
+    if (Tm::lane() == 0) flags[slot][Tm::warp()] = flag;
+  };
+  // what the list adds up to, warp by warp
+  auto list_sums = [&]() {
+    int all = 0;
+    for (int w = 0; w < list_warps; ++w) all |= flags[slot][w];
+    bad = all & 1;
+    if (all & 2) merge_list<kThreads>(p, idx, K);
+    if (Tm::warp() >= list_warps) return;
+    float top_lp = neg_inf(), top_z = neg_inf();
+#pragma unroll 1
+    for (int k = Tm::tid(); k < K; k += kThreads)
+      if (idx[k] >= 0) {
+        top_lp = fmaxf(top_lp, (float)p[k]);
+        top_z = fmaxf(top_z, zu[k]);
+      }
 #pragma unroll
     for (int w = 16; w > 0; w >>= 1) {
       top_lp = fmaxf(top_lp, __shfl_xor_sync(0xffffffffu, top_lp, w));
       top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
     }
-    const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (twice ? 2u : 0u));
-    if (Tm::lane() == 0) {
-      tops[slot][Tm::warp()][0] = top_lp;
-      tops[slot][Tm::warp()][1] = top_z;
-      flags[slot][Tm::warp()] = flag;
-    }
-  }
-  Tm::sync();
-  int all = 0;
-  top_lp = top_z = neg_inf();
-#pragma unroll 1
-  for (int w = 0; w < list_warps; ++w) {
-    top_lp = fmaxf(top_lp, tops[slot][w][0]);
-    top_z = fmaxf(top_z, tops[slot][w][1]);
-    all |= flags[slot][w];
-  }
-  bad = all & 1;
-  const double shift = o.renormalize && top_lp > neg_inf() ? (double)top_lp : 0.0;
-  if (all & 2) {                                  // an entry listed twice counts once
-    for (int k = Tm::tid(); k < K; k += kThreads) p[k] = idx[k] < 0 ? 0.0 : exp64(p[k] - shift);
-    Tm::sync();
-    if (Tm::tid() == 0)
-      for (int k = 0; k < K; ++k)
-        for (int q = k + 1; q < K; ++q)
-          if (idx[k] >= 0 && idx[q] == idx[k]) {
-            p[k] += p[q];
-            p[q] = 0.0;
-            idx[q] = -1;
-          }
-    Tm::sync();
-  }
-  if (Tm::warp() < list_warps) {
-    ListSums ls{0.0, 0.0, 0.0, 0.f};
+    if (!o.renormalize || top_lp == neg_inf()) top_lp = 0.f;
+    ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
 #pragma unroll 1
     for (int k = Tm::tid(); k < K; k += kThreads) {
       if (idx[k] < 0) continue;
-      const double lp = (all & 2) ? log(p[k]) : p[k] - shift;
-      const double pk = (all & 2) ? p[k] : exp64(lp);
+      const double lp = p[k] - (double)top_lp, pk = exp64(lp);
       const float zp = (zu[k] - top_z) * a.inv_t;
       p[k] = pk;
       ls.mass += pk;
@@ -1270,57 +1290,62 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       ls.e += __shfl_xor_sync(0xffffffffu, ls.e, w);
     }
     if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
-  }
+  };
   // the rest of the row
   Sums sum{neg_inf(), 0.f, 0.f};
-  constexpr int kStep = kThreads * N / 32;        // words of bits from one vector to the next
-  const uint32_t* my_bits = bits + 1 + (Tm::tid() * N >> 5);
-  const int my_shift = (Tm::tid() * N) & 31;
+  uint32_t now = chunk;
+  if (share.begin == share.end) {                 // no vector here: the list alone
+    Tm::sync();
+    mark();
+    Tm::sync();
+    list_sums();
+  }
 #pragma unroll 1
   for (int base = share.begin; base < share.end; base += cap) {
-    const int n = own_vectors<kThreads>(base, min(base + cap, share.end));
-    if (base != share.begin) st.copy(row, base, n);
-    const uint32_t* w = my_bits + (base - share.begin) * N / 32;
-    uint32_t at = st.buf;
-    int i = 0;
-#pragma unroll 1
-    for (int q = 0; q < 4; ++q) {
-      st.wait(q);
-#pragma unroll 1
-      for (int b = 0; b < st.per && i < n; ++b, i += kBatch) {
-        uint4 r[kBatch];
-        read_batch<kThreads>(at, r);
-        if (kMask) {
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u)
-            if (i + u < n) row.apply_mask(r[u], base + (i + u) * kThreads + Tm::tid());
-          write_batch<kThreads>(at, r);
-        }
-        constexpr uint32_t kOnes = (1u << N) - 1u;
-        uint32_t b4[kBatch], any = 0;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          b4[u] = w[u * kStep] >> my_shift;
-          any |= b4[u];
-        }
-        if (any & kOnes) {
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) drop_bits<T>(r[u], b4[u]);
-        }
-        w += kBatch * kStep;
-        at += kBatch * kThreads * 16;
-        typename Vec<T>::Max most = Vec<T>::wide_max(r[0]);
-#pragma unroll
-        for (int u = 1; u < kBatch; ++u) most = Vec<T>::larger(most, Vec<T>::wide_max(r[u]));
-        accumulate<T, kBatch, false, false>(r, Vec<T>::to_max(most), a.c, sum);
-      }
+    const int n = own_vectors<kThreads>(base, min(base + cap, share.end)), next = base + cap;
+    if (chunks > 1 && next < share.end) {
+      copy_chunk<T, kThreads>(2 * chunk + cap * 16 - now, row, next,
+                              own_vectors<kThreads>(next, min(next + cap, share.end)));
+      cp_async_wait<1>();
+    } else {
+      if (chunks == 1 && base != share.begin) copy_chunk<T, kThreads>(chunk, row, base, n);
+      cp_async_wait<0>();
     }
+    Tm::sync();                                   // the whole chunk is there
+    const int first = row.head + base * N, last = first + min(cap, share.end - base) * N;
+#pragma unroll 1
+    for (int k = Tm::tid(); k < K; k += kThreads) {
+      const int v = idx[k];
+      if (v >= first && v < last) sts_neg_inf<T>(now + (v - first) * (int)sizeof(T));
+    }
+    if (base == share.begin) mark();
+    Tm::sync();
+    if (base == share.begin) list_sums();
+    uint32_t at = now + Tm::tid() * 16;
+#pragma unroll 1
+    for (int i = 0; i < n; i += kBatch) {
+      uint4 r[kBatch];
+      read_batch<kThreads>(at, r);
+      if (kMask) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (i + u < n) row.apply_mask(r[u], base + (i + u) * kThreads + Tm::tid());
+        write_batch<kThreads>(at, r);
+      }
+      at += kBatch * kThreads * 16;
+      typename Vec<T>::Max most = Vec<T>::wide_max(r[0]);
+#pragma unroll
+      for (int u = 1; u < kBatch; ++u) most = Vec<T>::larger(most, Vec<T>::wide_max(r[u]));
+      accumulate<T, kBatch, false, false>(r, Vec<T>::to_max(most), a.c, sum);
+    }
+    if (chunks > 1) now = 2 * chunk + cap * 16 - now;
   }
   float edge = neg_inf();
   if (share.edge >= 0) {
     edge = row.at(share.edge);
-    const int u = share.edge - v0;
-    if (!((bits[u >> 5] >> (u & 31)) & 1u)) sum = join(sum, single(edge, a.c), a.c);
+    bool in = false;
+    for (int k = 0; k < K; ++k) in |= idx[k] == share.edge;
+    if (!in) sum = join(sum, single(edge, a.c), a.c);
   }
   sum = team_sums<kThreads>(sum, a.c, red[slot]);   // orders lred, too (a barrier, or one warp)
   if constexpr (kThreads == 32) __syncwarp();
@@ -1340,13 +1365,26 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
 #pragma unroll 1
       for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
     }
-    ListSums ls{0.0, 0.0, 0.0, 0.f};
+    // the warps' parts of the list, relative to the largest z and log P of all
+    float top_z = neg_inf(), top_lp = neg_inf();
+    for (int w = 0; w < list_warps; ++w) {
+      top_z = fmaxf(top_z, lred[slot][w].top_z);
+      if (lred[slot][w].mass > 0.0) top_lp = fmaxf(top_lp, lred[slot][w].top_lp);
+    }
+    ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
 #pragma unroll 1
     for (int w = 0; w < list_warps; ++w) {
-      ls.mass += lred[slot][w].mass;
-      ls.p_log_p += lred[slot][w].p_log_p;
-      ls.p_z += lred[slot][w].p_z;
-      ls.e += lred[slot][w].e;
+      const ListSums& b = lred[slot][w];
+      const double up = b.mass > 0.0 ? (double)b.top_lp - (double)top_lp : 0.0;
+      const double f = up == 0.0 ? 1.0 : exp64(up);
+      const float zp = b.top_z == neg_inf() ? 0.f : (b.top_z - top_z) * a.inv_t;
+      if (Tm::lane() == 0) factor[slot][w] = (float)f;
+      ls.mass += f * b.mass;
+      if (b.mass > 0.0) {
+        ls.p_log_p += f * (b.p_log_p + up * b.mass);
+        ls.p_z += f * (b.p_z + (double)zp * b.mass);
+      }
+      ls.e += b.e * (zp == 0.f ? 1.f : expf(zp));
     }
     const bool rest = sum.m != neg_inf(), listed = top_z != neg_inf();
     bad |= sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
@@ -1400,10 +1438,10 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     for (int base = share.begin; base < share.end; base += cap) {
       const int n = own_vectors<kThreads>(base, min(base + cap, share.end));
       if (!one) {
-        st.copy(row, base, n);
+        copy_chunk<T, kThreads>(chunk, row, base, n);
         cp_async_wait<0>();
       }
-      uint32_t at = st.buf;
+      uint32_t at = chunk + Tm::tid() * 16;
       int j = base + Tm::tid();
 #pragma unroll 1
       for (int i = 0; i < n; i += kBatch) {
@@ -1432,7 +1470,8 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     const int v = idx[k];
     if (v < share.first || v >= share.last) continue;
     const float q = expf((zu[k] - d.big) * a.inv_t) / d.norm;
-    row.grad[v] = to_type<T>(d.nan + d.scale * (q - (float)p[k] * d.inv));
+    const float pk = (float)p[k] * factor[slot][Tm::warp()];
+    row.grad[v] = to_type<T>(d.nan + d.scale * (q - pk * d.inv));
   }
 }
 

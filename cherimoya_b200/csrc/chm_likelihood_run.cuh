@@ -118,13 +118,20 @@ int run_log_probs_grad(const Rows& a, const ScoreGradArgs& o, long long n, cudaS
 template <typename T, bool kMask>
 int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t st) {
   const int nvec = largest(a) / Vec<T>::N;
-  const Cut c = cut_rows(nvec, n, o.n_listed <= 128);
-  const int team =
-      distill_bytes(o.n_listed, c.cap, (nvec >> c.log_blocks) + 1, Vec<T>::N);
+  Cut c = cut_rows(nvec, n, o.n_listed <= 128);
+  int chunks = 1;
+  if (!a.grad && nvec > 4096) {
+    // nothing is looked at twice: two chunks of 32 KB in turn, by one block where rows abound
+    c = {256, 0, 2048};
+    while (c.log_blocks < 3 && n << c.log_blocks < 3 * 148 && nvec >> c.log_blocks > 4096)
+      ++c.log_blocks;
+    chunks = 2;
+  }
+  const int team = distill_bytes(o.n_listed, c.cap, chunks, largest(a));
   const size_t smem = (size_t)(c.threads == 32 ? 4 : 1) * team;
   auto run = [&](auto kernel) {
     return launch(kernel, c.threads, c.log_blocks, n, smem, st, true, a, o, (unsigned)n,
-                  c.log_blocks, c.cap, team);
+                  c.log_blocks, c.cap, chunks, team);
   };
   switch (c.threads) {
     case 32: return run(distill_kernel<T, 32, kMask>);

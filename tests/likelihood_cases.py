@@ -120,7 +120,8 @@ def case_distill(dev, shape, groups, dtype, k, renorm, T, mask, weight, seed=1):
         C.check_distill(z, idx, lp, renorm, m, groups, T, w, reduction, loss, grad)
     with torch.no_grad():
         again = cb.distillation_loss(z, idx, lp, reduction="none", **how)
-    assert torch.equal(again, loss)
+    # without a gradient long rows are cut otherwise: the same bound, not the same bits
+    C.check_distill(z, idx, lp, renorm, m, groups, T, w, "none", again, None)
     up = torch.randn(lead, generator=g).to(dev)
     loss = cb.distillation_loss(z, idx, lp, reduction="none", **how)
     auto, = torch.autograd.grad(loss, z, up)
