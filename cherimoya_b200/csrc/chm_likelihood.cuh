@@ -1124,6 +1124,75 @@ struct ListSums {
   float e;                         // sum exp(z')
   float top_z, top_lp;             // the warp's largest z, log P: z' and P are relative to them
 };
+// What a warp's part of the list adds up to; p becomes P from log P.
+template <int kThreads>
+__device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int* idx, int K,
+                                           int renormalize, float inv_t) {
+  float top_lp = neg_inf(), top_z = neg_inf();
+#pragma unroll 1
+  for (int k = Team<kThreads>::tid(); k < K; k += kThreads)
+    if (idx[k] >= 0) {
+      top_lp = fmaxf(top_lp, (float)p[k]);
+      top_z = fmaxf(top_z, zu[k]);
+    }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) {
+    top_lp = fmaxf(top_lp, __shfl_xor_sync(0xffffffffu, top_lp, w));
+    top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
+  }
+  if (!renormalize || top_lp == neg_inf()) top_lp = 0.f;
+  ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
+#pragma unroll 1
+  for (int k = Team<kThreads>::tid(); k < K; k += kThreads) {
+    if (idx[k] < 0) continue;
+    const double lp = p[k] - (double)top_lp, pk = exp64(lp);
+    const float zp = (zu[k] - top_z) * inv_t;
+    p[k] = pk;
+    ls.mass += pk;
+    if (pk > 0.0) {
+      ls.p_log_p += pk * lp;
+      ls.p_z += pk * (double)zp;
+    }
+    ls.e += expf(zp);
+  }
+#pragma unroll 1
+  for (int w = 16; w > 0; w >>= 1) {
+    ls.mass += __shfl_xor_sync(0xffffffffu, ls.mass, w);
+    ls.p_log_p += __shfl_xor_sync(0xffffffffu, ls.p_log_p, w);
+    ls.p_z += __shfl_xor_sync(0xffffffffu, ls.p_z, w);
+    ls.e += __shfl_xor_sync(0xffffffffu, ls.e, w);
+  }
+  return ls;
+}
+
+// The warps' parts of the list, relative to the largest z and log P of all, as
+// the first one's; factor: of each warp's P to the common ones. One warp.
+template <int kThreads>
+__device__ __noinline__ void join_list(ListSums* part, float* factor, int warps, float inv_t) {
+  float top_z = neg_inf(), top_lp = neg_inf();
+  for (int w = 0; w < warps; ++w) {
+    top_z = fmaxf(top_z, part[w].top_z);
+    if (part[w].mass > 0.0) top_lp = fmaxf(top_lp, part[w].top_lp);
+  }
+  ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
+#pragma unroll 1
+  for (int w = 0; w < warps; ++w) {
+    const ListSums b = part[w];
+    const double up = b.mass > 0.0 ? (double)b.top_lp - (double)top_lp : 0.0;
+    const double f = up == 0.0 ? 1.0 : exp64(up);
+    const float zp = b.top_z == neg_inf() ? 0.f : (b.top_z - top_z) * inv_t;
+    if (Team<kThreads>::lane() == 0) factor[w] = (float)f;
+    ls.mass += f * b.mass;
+    if (b.mass > 0.0) {
+      ls.p_log_p += f * (b.p_log_p + up * b.mass);
+      ls.p_z += f * (b.p_z + (double)zp * b.mass);
+    }
+    ls.e += b.e * (zp == 0.f ? 1.f : expf(zp));
+  }
+  __syncwarp();
+  if (warps > 0 && Team<kThreads>::lane() == 0) part[0] = ls;
+}
+
 // A list in which an entry may be twice: the first one takes the others' mass
 // (p: log P before and after), the others leave the list. Marks can coincide
 // without a repeat, so most calls find none.
@@ -1160,12 +1229,6 @@ __device__ __noinline__ void merge_list(double* p, int* idx, int K) {
   Tm::sync();
 }
 
-// What every thread needs to know of the row for its gradient.
-struct DistillRow {
-  float coef, ref, nan;            // nan: 0, or NaN for a row without a distribution
-  float scale, big, norm, inv;     // of the listed entries
-};
-
 // The list's entries are overwritten by -inf in shared memory before the one
 // pass over the row, so that pass gives maximum and sum over the rest alone,
 // without a difference of nearly equal numbers; the teacher's masses are added
@@ -1186,7 +1249,6 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   __shared__ ListSums lred[Tm::kPerBlock][Tm::kWarps];
   __shared__ float factor[Tm::kPerBlock][Tm::kWarps];   // of a warp's p, to that of all
   __shared__ int flags[Tm::kPerBlock][Tm::kWarps];
-  __shared__ DistillRow done[Tm::kPerBlock];
   __shared__ float cl[kMaxCluster][2];            // every block's maximum and sum
   const int slot = Tm::slot(), K = o.n_listed;
   const int blocks = 1 << log_blocks, rank = blockIdx.x & (blocks - 1);
@@ -1223,7 +1285,9 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   if (o.upstream) weight *= o.upstream[row.index * o.upstream_stride];
   const int words = seen_words(row.size);
   for (int w = Tm::tid(); w < words; w += kThreads) seen[w] = 0u;
+  const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
   bool bad = false;
+  // While the row is on its way: the list, an entry to a thread.
 #pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
     const long long i = o.indices[row.index * K + k];
@@ -1235,11 +1299,18 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     zu[k] = z;
     p[k] = (double)lp;
   }
-  const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
-  // marks the list's entries, to see whether one is there twice
-  auto mark = [&]() {
-    if (Tm::warp() >= list_warps) return;
-    bool again = false;
+  typename Row<T>::MaskBytes ahead[kBatch];       // the first batch's mask
+  auto fetch_mask = [&](int base, int i, int n) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (i + u < n) ahead[u] = row.mask_bytes(base + (i + u) * kThreads + Tm::tid());
+  };
+  if (kMask)
+    fetch_mask(share.begin, 0,
+               own_vectors<kThreads>(share.begin, min(share.begin + cap, share.end)));
+  Tm::sync();                                     // the marks are clear
+  if (Tm::warp() < list_warps) {
+    bool again = false;                           // is an entry there twice? (or seems to be)
 #pragma unroll 1
     for (int k = Tm::tid(); k < K; k += kThreads) {
       const int v = idx[k] & (kSeenBits - 1);
@@ -1247,61 +1318,14 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     }
     const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (again ? 2u : 0u));
     if (Tm::lane() == 0) flags[slot][Tm::warp()] = flag;
-  };
-  // what the list adds up to, warp by warp
-  auto list_sums = [&]() {
-    int all = 0;
-    for (int w = 0; w < list_warps; ++w) all |= flags[slot][w];
-    bad = all & 1;
-    if (all & 2) merge_list<kThreads>(p, idx, K);
-    if (Tm::warp() >= list_warps) return;
-    float top_lp = neg_inf(), top_z = neg_inf();
-#pragma unroll 1
-    for (int k = Tm::tid(); k < K; k += kThreads)
-      if (idx[k] >= 0) {
-        top_lp = fmaxf(top_lp, (float)p[k]);
-        top_z = fmaxf(top_z, zu[k]);
-      }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) {
-      top_lp = fmaxf(top_lp, __shfl_xor_sync(0xffffffffu, top_lp, w));
-      top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
-    }
-    if (!o.renormalize || top_lp == neg_inf()) top_lp = 0.f;
-    ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
-#pragma unroll 1
-    for (int k = Tm::tid(); k < K; k += kThreads) {
-      if (idx[k] < 0) continue;
-      const double lp = p[k] - (double)top_lp, pk = exp64(lp);
-      const float zp = (zu[k] - top_z) * a.inv_t;
-      p[k] = pk;
-      ls.mass += pk;
-      if (pk > 0.0) {
-        ls.p_log_p += pk * lp;
-        ls.p_z += pk * (double)zp;
-      }
-      ls.e += expf(zp);
-    }
-#pragma unroll 1
-    for (int w = 16; w > 0; w >>= 1) {
-      ls.mass += __shfl_xor_sync(0xffffffffu, ls.mass, w);
-      ls.p_log_p += __shfl_xor_sync(0xffffffffu, ls.p_log_p, w);
-      ls.p_z += __shfl_xor_sync(0xffffffffu, ls.p_z, w);
-      ls.e += __shfl_xor_sync(0xffffffffu, ls.e, w);
-    }
+    const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, a.inv_t);
     if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
-  };
+  }
   // the rest of the row
   Sums sum{neg_inf(), 0.f, 0.f};
   uint32_t now = chunk;
-  if (share.begin == share.end) {                 // no vector here: the list alone
-    Tm::sync();
-    mark();
-    Tm::sync();
-    list_sums();
-  }
 #pragma unroll 1
-  for (int base = share.begin; base < share.end; base += cap) {
+  for (int base = share.begin; base < share.end || base == share.begin; base += cap) {
     const int n = own_vectors<kThreads>(base, min(base + cap, share.end)), next = base + cap;
     if (chunks > 1 && next < share.end) {
       copy_chunk<T, kThreads>(2 * chunk + cap * 16 - now, row, next,
@@ -1311,6 +1335,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       if (chunks == 1 && base != share.begin) copy_chunk<T, kThreads>(chunk, row, base, n);
       cp_async_wait<0>();
     }
+    if (kMask && base != share.begin) fetch_mask(base, 0, n);
     Tm::sync();                                   // the whole chunk is there
     const int first = row.head + base * N, last = first + min(cap, share.end - base) * N;
 #pragma unroll 1
@@ -1318,9 +1343,9 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       const int v = idx[k];
       if (v >= first && v < last) sts_neg_inf<T>(now + (v - first) * (int)sizeof(T));
     }
-    if (base == share.begin) mark();
+    if (base == share.begin && Tm::warp() == Tm::kWarps - 1)
+      join_list<kThreads>(lred[slot], factor[slot], list_warps, a.inv_t);
     Tm::sync();
-    if (base == share.begin) list_sums();
     uint32_t at = now + Tm::tid() * 16;
 #pragma unroll 1
     for (int i = 0; i < n; i += kBatch) {
@@ -1329,7 +1354,8 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       if (kMask) {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
-          if (i + u < n) row.apply_mask(r[u], base + (i + u) * kThreads + Tm::tid());
+          if (i + u < n) Row<T>::apply_mask(r[u], ahead[u]);
+        fetch_mask(base, i + kBatch, n);
         write_batch<kThreads>(at, r);
       }
       at += kBatch * kThreads * 16;
@@ -1347,6 +1373,20 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     for (int k = 0; k < K; ++k) in |= idx[k] == share.edge;
     if (!in) sum = join(sum, single(edge, a.c), a.c);
   }
+  int all = 0;
+  for (int w = 0; w < list_warps; ++w) all |= flags[slot][w];
+  if (all & 2) {                                  // an entry listed twice counts once
+    for (int k = Tm::tid(); k < K; k += kThreads) p[k] = (double)o.log_probs[row.index * K + k];
+    Tm::sync();
+    merge_list<kThreads>(p, idx, K);
+    if (Tm::warp() < list_warps) {
+      const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, a.inv_t);
+      if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
+    }
+    Tm::sync();
+    if (Tm::warp() == 0) join_list<kThreads>(lred[slot], factor[slot], list_warps, a.inv_t);
+    Tm::sync();
+  }
   sum = team_sums<kThreads>(sum, a.c, red[slot]);   // orders lred, too (a barrier, or one warp)
   if constexpr (kThreads == 32) __syncwarp();
   if (blocks > 1) {
@@ -1357,70 +1397,44 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     }
     cluster_arrive();
     cluster_wait();
-  }
-  if (Tm::warp() == 0) {
-    // one warp for all: loss and coefficients
-    if (blocks > 1) {
-      sum = {cl[0][0], cl[0][1], 0.f};
+    sum = {cl[0][0], cl[0][1], 0.f};
 #pragma unroll 1
-      for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
-    }
-    // the warps' parts of the list, relative to the largest z and log P of all
-    float top_z = neg_inf(), top_lp = neg_inf();
-    for (int w = 0; w < list_warps; ++w) {
-      top_z = fmaxf(top_z, lred[slot][w].top_z);
-      if (lred[slot][w].mass > 0.0) top_lp = fmaxf(top_lp, lred[slot][w].top_lp);
-    }
-    ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
-#pragma unroll 1
-    for (int w = 0; w < list_warps; ++w) {
-      const ListSums& b = lred[slot][w];
-      const double up = b.mass > 0.0 ? (double)b.top_lp - (double)top_lp : 0.0;
-      const double f = up == 0.0 ? 1.0 : exp64(up);
-      const float zp = b.top_z == neg_inf() ? 0.f : (b.top_z - top_z) * a.inv_t;
-      if (Tm::lane() == 0) factor[slot][w] = (float)f;
-      ls.mass += f * b.mass;
-      if (b.mass > 0.0) {
-        ls.p_log_p += f * (b.p_log_p + up * b.mass);
-        ls.p_z += f * (b.p_z + (double)zp * b.mass);
-      }
-      ls.e += b.e * (zp == 0.f ? 1.f : expf(zp));
-    }
-    const bool rest = sum.m != neg_inf(), listed = top_z != neg_inf();
-    bad |= sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
-    const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
-    const double inv = whole && ls.mass > 0.0 ? 1.0 / ls.mass : 1.0;
-    const float p_r = whole ? 0.f : (float)(1.0 - ls.mass);
-    const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
-    // the two normalisers relative to the larger of the two maxima
-    const float big = fmaxf(rest ? sum.m : neg_inf(), top_z);
-    const float down_r = rest ? (sum.m - big) * a.inv_t : 0.f;
-    const float down_u = listed ? (top_z - big) * a.inv_t : 0.f;
-    const float norm_r = rest ? sum.s * expf(down_r) : 0.f;
-    const float norm = norm_r + (listed ? ls.e * expf(down_u) : 0.f);
-    if (rank == 0 && Tm::tid() == 0 && o.row_loss) {
-      const float log_all = logf(norm);
-      double loss = 0.0;
-      if (live && ls.mass > 0.0)
-        loss = inv * (ls.p_log_p - ls.p_z + ((double)log_all - (double)down_u) * ls.mass) +
-               (whole ? log(inv) * (inv * ls.mass) : 0.0);
-      if (live && p_r > 0.f)
-        loss += (double)p_r * ((double)logf(p_r) -
-                               ((double)down_r + (double)logf(sum.s) - (double)log_all));
-      o.row_loss[row.index] =
-          bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
-    }
-    if (Tm::tid() == 0) {
-      const float scale = live ? weight * a.t : 0.f;
-      const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
-      done[slot] = {coef, rest ? sum.m : 0.f, bad || coef != coef ? quiet_nan() : 0.f,
-                    scale, big, norm, (float)inv};
-    }
+    for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
   }
-  if (!row.grad) return;
-  Tm::sync();
-  const DistillRow d = done[slot];
-  const float2 nref = {-d.ref, -d.ref}, cc = {a.c, a.c}, kk = {d.coef, d.coef};
+  const ListSums ls = K > 0 ? lred[slot][0] : ListSums{0.0, 0.0, 0.0, 0.f, neg_inf(), 0.f};
+  const bool rest = sum.m != neg_inf(), listed = ls.top_z != neg_inf();
+  bad = (all & 1) || sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
+  const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
+  const float inv = whole && ls.mass > 0.0 ? 1.f / (float)ls.mass : 1.f;
+  const float p_r = whole ? 0.f : (float)(1.0 - ls.mass);
+  const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
+  // the two normalisers relative to the larger of the two maxima
+  const float big = fmaxf(rest ? sum.m : neg_inf(), ls.top_z);
+  const float down_r = rest ? (sum.m - big) * a.inv_t : 0.f;
+  const float down_u = listed ? (ls.top_z - big) * a.inv_t : 0.f;
+  const float norm_r = rest ? sum.s * expf(down_r) : 0.f;
+  const float norm = norm_r + (listed ? ls.e * expf(down_u) : 0.f);
+  auto write_loss = [&]() {                       // by one thread, when the others are done
+    if (rank != 0 || Tm::tid() != kThreads - 1 || !o.row_loss) return;
+    const double log_all = logf(norm);
+    double loss = 0.0;
+    if (live && ls.mass > 0.0) {
+      loss = ls.p_log_p - ls.p_z + (log_all - (double)down_u) * ls.mass;
+      if (whole) loss = loss / ls.mass - log(ls.mass);
+    }
+    if (live && p_r > 0.f)
+      loss += (double)p_r * ((double)logf(p_r) - ((double)down_r + (double)logf(sum.s) - log_all));
+    o.row_loss[row.index] =
+        bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
+  };
+  if (!row.grad) {
+    write_loss();
+    return;
+  }
+  const float scale = live ? weight * a.t : 0.f, ref = rest ? sum.m : 0.f;
+  const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
+  const float nan = bad || coef != coef ? quiet_nan() : 0.f;   // of a row without a distribution
+  const float2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
   auto slope = [&](const uint4& r, int j) {
     float z[N];
     Vec<T>::unpack(r, z);
@@ -1433,7 +1447,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     }
     row.store(j, z, vec_store);
   };
-  if (d.nan == 0.f) {
+  if (nan == 0.f) {
 #pragma unroll 1
     for (int base = share.begin; base < share.end; base += cap) {
       const int n = own_vectors<kThreads>(base, min(base + cap, share.end));
@@ -1462,17 +1476,17 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   }
   if (share.edge >= 0)
     row.grad[share.edge] =
-        to_type<T>(edge == neg_inf() ? 0.f : d.nan + ex2((edge - d.ref) * a.c) * d.coef);
-  if (K == 0) return;
-  Tm::sync();                                     // the listed entries are written again
+        to_type<T>(edge == neg_inf() ? 0.f : nan + ex2((edge - ref) * a.c) * coef);
+  if (K > 0) Tm::sync();                          // the listed entries are written again
 #pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
     const int v = idx[k];
     if (v < share.first || v >= share.last) continue;
-    const float q = expf((zu[k] - d.big) * a.inv_t) / d.norm;
+    const float q = expf((zu[k] - big) * a.inv_t) / norm;
     const float pk = (float)p[k] * factor[slot][Tm::warp()];
-    row.grad[v] = to_type<T>(d.nan + d.scale * (q - pk * d.inv));
+    row.grad[v] = to_type<T>(nan + scale * (q - pk * inv));
   }
+  write_loss();
 }
 
 // Sum of the rows' losses by one block, in 64 bits and a fixed order.

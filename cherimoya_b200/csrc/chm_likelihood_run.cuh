@@ -30,7 +30,7 @@ Cut cut_rows(int nvec, long long rows, bool warp) {
   while (c.log_blocks < 3 && rows << c.log_blocks < 2 * 148 && nvec > 512 << c.log_blocks)
     ++c.log_blocks;
   const int share = (nvec + (1 << c.log_blocks) - 1) >> c.log_blocks;
-  c.threads = warp && share <= 64 ? 32 : share <= 1024 ? 128 : share <= 4096 ? 256 : 512;
+  c.threads = warp && share <= 256 ? 32 : share <= 1024 ? 128 : share <= 4096 ? 256 : 512;
   if (c.log_blocks && c.threads < 256) c.threads = 256;
   const int most = std::min(std::max(share, 1), kChunkBytes / 16);
   c.cap = (most + kBatch * c.threads - 1) / (kBatch * c.threads) * (kBatch * c.threads);
