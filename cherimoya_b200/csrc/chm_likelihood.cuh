@@ -1238,8 +1238,10 @@ __device__ __noinline__ void merge_list(double* p, int* idx, int K) {
 //   dz_u = T w (exp(z'_u - lse) - P_u)              in it
 // so the gradient is one more exponential per entry in shared memory. Without
 // a gradient the chunks are small and there are two, one on its way.
+// At least three blocks of 256 to an SM, which 64 KB of shared memory allow.
 template <typename T, int kThreads, bool kMask>
-__global__ void __launch_bounds__(Team<kThreads>::kBlock)
+__global__ void
+__launch_bounds__(Team<kThreads>::kBlock, kThreads == 512 ? 1 : kThreads == 256 ? 3 : 5)
 distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned rows, int log_blocks,
                int cap, int chunks, int team_bytes) {
   using Tm = Team<kThreads>;

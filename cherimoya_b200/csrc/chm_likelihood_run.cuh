@@ -3,6 +3,7 @@
 #pragma once
 #include <algorithm>
 #include <climits>
+#include <vector>
 
 #include "../../include/cherimoya_b200.h"
 #include "chm_host.h"
@@ -48,16 +49,40 @@ Cut cut_stream(int nvec, long long rows, int top_k) {
   return c;
 }
 
+// Lets a kernel use all the dynamic shared memory that the current device has
+// for a block; asked once per kernel, device and thread.
+int lift_smem_limit(const void* kernel) {
+  struct Known {
+    const void* kernel;
+    int device;
+  };
+  thread_local std::vector<Known> known;
+  int device = 0, limit = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return CHM_ERR_CUDA;
+  for (const Known& k : known)
+    if (k.kernel == kernel && k.device == device) return CHM_OK;
+  cudaFuncAttributes attr;
+  if (cudaDeviceGetAttribute(&limit, cudaDevAttrMaxSharedMemoryPerBlockOptin, device) !=
+          cudaSuccess ||
+      cudaFuncGetAttributes(&attr, kernel) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           limit - (int)attr.sharedSizeBytes) != cudaSuccess)
+    return CHM_ERR_CUDA;
+  known.push_back({kernel, device});
+  return CHM_OK;
+}
+
+// Launches a kernel with a team, or a cluster of blocks, for each row.
 template <typename... KArgs, typename... Args>
 int launch(void (*kernel)(KArgs...), int threads, int log_blocks, long long rows, size_t smem,
            cudaStream_t st, bool cluster, Args... args) {
   const int per_block = threads == 32 ? 4 : 1, blocks = 1 << log_blocks;
   const long long grid = (rows + per_block - 1) / per_block * blocks;
   if (grid > INT_MAX) return CHM_ERR_UNSUPPORTED;
-  if (smem > 32 << 10 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-          cudaSuccess)
-    return CHM_ERR_CUDA;
+  if (smem > 16 << 10) {
+    const int status = lift_smem_limit(reinterpret_cast<const void*>(kernel));
+    if (status != CHM_OK) return status;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(threads * per_block);
@@ -103,7 +128,8 @@ int run_log_probs_grad_m(const Rows& a, const ScoreGradArgs& o, long long n, cud
   const int spots = o.n_targets * (o.g_log_probs != nullptr) + o.top_k * (o.g_top != nullptr);
   const size_t smem = (size_t)(threads == 32 ? 4 : 1) * spots * 8;
   auto run = [&](auto kernel) {
-    return launch(kernel, threads, log_blocks, n, smem, st, false, a, o, (unsigned)n, log_blocks);
+    return launch(kernel, threads, log_blocks, n, smem, st, false, a, o, (unsigned)n,
+                  log_blocks);
   };
   return threads == 32 ? run(log_probs_grad_kernel<T, 32, kMask>)
                        : run(log_probs_grad_kernel<T, 256, kMask>);

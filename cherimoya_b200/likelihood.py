@@ -55,74 +55,38 @@ class ProfileLogProbs(NamedTuple):
     top_indices: torch.Tensor      # (*lead, top_k) int64
 
 
-class _Layout(NamedTuple):
-    """Where the rows are: n examples, per group its first element and its size."""
-    lead: tuple
-    n: int
-    stride: int
-    offsets: tuple
-    sizes: tuple
-
-
 def _fail(text):
     raise RuntimeError("cherimoya_b200: " + text)
 
 
-@functools.lru_cache(maxsize=256)
-def _group_layout(groups, width, channel_stride):
-    _validate_signal_groups(list(groups))
-    offsets, first = [], 0
-    for g in groups:
-        offsets.append(first * channel_stride)
-        first += g
-    return tuple(offsets), tuple(g * width for g in groups)
-
-
-def _place(x, groups):
-    """(x, or a contiguous copy where its strides have no such rows; its layout)."""
+@functools.lru_cache(maxsize=1024)
+def _check_shape(shape, groups):
+    """The shape of the per-row results; groups: None, or a tuple."""
     if groups is None:
-        width, lead = x.shape[-1], tuple(x.shape[:-1])
-        if x.dim() != 2:
-            x = x.reshape(_numel(lead), width)
-        if width > 1 and x.stride(1) != 1:
-            x = x.contiguous()
-        return x, _Layout(lead, x.shape[0], x.stride(0), (0,), (width,))
-    n, _, width = x.shape
-    whole = all(g == 1 for g in groups)
-    if (width > 1 and x.stride(2) != 1) or not (whole or x.stride(1) == width):
-        x = x.contiguous()
-    offsets, sizes = _group_layout(groups, width, x.stride(1))
-    return x, _Layout((n, len(groups)), n, x.stride(0), offsets, sizes)
-
-
-def _numel(shape):
-    n = 1
-    for s in shape:
-        n *= s
-    return n
+        if len(shape) < 1:
+            _fail("logits need at least one axis")
+        lead, largest = shape[:-1], shape[-1]
+    else:
+        if len(shape) != 3:
+            _fail("logits with signal_groups must be (N, n_outputs, W), got {}".format(
+                tuple(shape)))
+        _validate_signal_groups(list(groups))
+        if sum(groups) != shape[1]:
+            _fail("signal_groups {} do not add up to the {} channels of the logits".format(
+                list(groups), shape[1]))
+        lead, largest = (shape[0], len(groups)), max(groups) * shape[2]
+    if largest > MAX_ENTRIES:
+        _fail("a row has {} cells; at most {} are supported".format(largest, MAX_ENTRIES))
+    return tuple(lead)
 
 
 def _check(logits, mask, signal_groups, temperature):
+    """(groups as a tuple, empty for none; the mask in the logits' shape; the rows' shape)"""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
         _fail("logits must be a float32, bfloat16 or float16 tensor, got {}".format(
             getattr(logits, "dtype", type(logits).__name__)))
-    groups = None
-    if signal_groups is not None:
-        groups = tuple(signal_groups)
-        if logits.dim() != 3:
-            _fail("logits with signal_groups must be (N, n_outputs, W), got {}".format(
-                tuple(logits.shape)))
-        _group_layout(groups, 1, 1)
-        if sum(groups) != logits.shape[1]:
-            _fail("signal_groups {} do not add up to the {} channels of the logits".format(
-                list(groups), logits.shape[1]))
-        largest = max(groups) * logits.shape[2]
-    else:
-        if logits.dim() < 1:
-            _fail("logits need at least one axis")
-        largest = logits.shape[-1]
-    if largest > MAX_ENTRIES:
-        _fail("a row has {} cells; at most {} are supported".format(largest, MAX_ENTRIES))
+    groups = None if signal_groups is None else tuple(signal_groups)
+    lead = _check_shape(logits.shape, groups)
     if not _MIN_T <= temperature <= _MAX_T:
         raise ValueError("temperature must be between 1/1024 and 1024, got {!r}".format(
             temperature))
@@ -137,13 +101,13 @@ def _check(logits, mask, signal_groups, temperature):
             except RuntimeError:
                 _fail("mask of shape {} does not broadcast to the logits' {}".format(
                     tuple(mask.shape), tuple(logits.shape)))
-    return groups, mask
+    return groups or (), mask, lead
 
 
-def _check_list(t, name, lead, device, count):
+def _check_list(t, name, lead, device):
     if t.dtype not in (torch.int64, torch.int32):
         _fail("{} must be int64 or int32, got {}".format(name, t.dtype))
-    if tuple(t.shape[:-1]) != lead or t.dim() != len(lead) + 1:
+    if t.dim() != len(lead) + 1 or t.shape[:-1] != lead:
         _fail("{} must have the shape {} + (count,), got {}".format(name, lead, tuple(t.shape)))
     if t.device != device:
         _fail("{} must be on the logits' device".format(name))
@@ -154,27 +118,44 @@ def _check_list(t, name, lead, device, count):
 
 
 # ------------------------------------------------------------ CPU formulas
-def _cpu_rows(z, mask, lay, temperature):
-    """Rows padded to the widest group: logits (R, V) fp32 with -inf outside, in example order."""
-    width = max(lay.sizes, default=0)
-    out = torch.full((lay.n, len(lay.sizes), width), float("-inf"), dtype=torch.float32)
-    for g, (o, s) in enumerate(zip(lay.offsets, lay.sizes)):
-        v = torch.as_strided(z, (lay.n, s), (lay.stride, 1), z.storage_offset() + o).float()
-        if mask is not None:
-            m, ml = mask
-            v = v.masked_fill(~torch.as_strided(m, (lay.n, s), (ml.stride, 1),
-                                                m.storage_offset() + ml.offsets[g]),
-                              float("-inf"))
-        out[:, g, :s] = v
-    sizes = torch.tensor(lay.sizes).expand(lay.n, -1).reshape(-1)
-    return out.reshape(lay.n * len(lay.sizes), width), sizes
+def _lead_rows(x):
+    n = 1
+    for extent in x.shape[:-1]:
+        n *= extent
+    return n
 
 
-def _cpu_write(grad, rows, glay):
-    rows = rows.reshape(glay.n, len(glay.sizes), rows.shape[-1])
-    for g, (o, s) in enumerate(zip(glay.offsets, glay.sizes)):
-        torch.as_strided(grad, (glay.n, s), (glay.stride, 1),
-                         grad.storage_offset() + o).copy_(rows[:, g, :s])
+def _cpu_rows(logits, mask, groups):
+    """Rows padded to the widest group, example by example: logits (R, V) fp32 with -inf where
+    no entry takes part, and each row's size."""
+    z = logits.detach().float()
+    if mask is not None:
+        z = z.masked_fill(~mask, float("-inf"))
+    width = z.shape[-1]
+    sizes = [g * width for g in groups] or [width]
+    n = z.shape[0] if groups else _lead_rows(z)
+    out = torch.full((n, len(sizes), max(sizes)), float("-inf"))
+    first = 0
+    for i, size in enumerate(sizes):
+        if groups:
+            part = z[:, first:first + groups[i]].reshape(n, size)
+            first += groups[i]
+        else:
+            part = z.reshape(n, size)
+        out[:, i, :size] = part
+    return (out.reshape(n * len(sizes), max(sizes)),
+            torch.tensor(sizes).expand(n, -1).reshape(-1))
+
+
+def _cpu_write(logits, rows, groups):
+    """A gradient of the logits' shape and type from padded rows."""
+    width = logits.shape[-1]
+    if not groups:
+        return rows.reshape(logits.shape).to(logits.dtype)
+    n = logits.shape[0]
+    rows = rows.reshape(n, len(groups), rows.shape[-1])
+    parts = [rows[:, i, :g * width].reshape(n, g, width) for i, g in enumerate(groups)]
+    return torch.cat(parts, 1).to(logits.dtype)
 
 
 def _cpu_max(z):
@@ -193,8 +174,8 @@ def _cpu_gather(z, idx, sizes):
     return torch.where((idx < 0) | past, float("-inf"), got), past
 
 
-def _cpu_log_probs(z, mask, lay, targets, top_k, temperature):
-    z, sizes = _cpu_rows(z, mask, lay, temperature)
+def _cpu_log_probs(logits, mask, groups, targets, top_k, temperature):
+    z, sizes = _cpu_rows(logits, mask, groups)
     R = z.shape[0]
     m = _cpu_max(z)
     x = (z - m) / temperature
@@ -222,9 +203,9 @@ def _cpu_log_probs(z, mask, lay, targets, top_k, temperature):
     return lp, h, (m / temperature + log_s).reshape(R), top, at, stats
 
 
-def _cpu_log_probs_backward(z, mask, lay, targets, top_indices, stats, entropy, g_lp, g_h, g_norm,
-                            g_top, temperature, grad, glay):
-    z, sizes = _cpu_rows(z, mask, lay, temperature)
+def _cpu_log_probs_backward(logits, mask, groups, targets, top_indices, stats, entropy, g_lp, g_h,
+                            g_norm, g_top, temperature):
+    z, sizes = _cpu_rows(logits, mask, groups)
     R = z.shape[0]
     m, log_s = stats[:, :1], stats[:, 1:]
     lists = [(i.reshape(R, i.shape[-1]), g.reshape(R, i.shape[-1])) for i, g in ((targets, g_lp), (top_indices, g_top))
@@ -244,12 +225,12 @@ def _cpu_log_probs_backward(z, mask, lay, targets, top_indices, stats, entropy, 
     if idx.shape[1] and z.shape[1]:
         d.scatter_add_(-1, idx.clamp(0, z.shape[1] - 1),
                        torch.where((idx < 0) | past, 0.0, g))
-    _cpu_write(grad, torch.where(z == float("-inf"), 0.0, d / temperature), glay)
+    return _cpu_write(logits, torch.where(z == float("-inf"), 0.0, d / temperature), groups)
 
 
-def _cpu_distill(z, mask, lay, idx, t_lp, renormalize, weight, scale, upstream, temperature, grad,
-                 glay):
-    z, sizes = _cpu_rows(z, mask, lay, temperature)
+def _cpu_distill(logits, mask, groups, idx, t_lp, renormalize, weight, scale, upstream,
+                 want_grad, temperature):
+    z, sizes = _cpu_rows(logits, mask, groups)
     R, V = z.shape
     inf = float("inf")
     w = torch.ones(R, 1) if weight is None else weight.reshape(R, 1)
@@ -297,47 +278,36 @@ def _cpu_distill(z, mask, lay, idx, t_lp, renormalize, weight, scale, upstream, 
     loss = torch.where(live, loss, 0.0) * temperature ** 2 * w
     loss = torch.where(bad, float("nan"), loss)
     loss = torch.where(skip, 0.0, loss)
-    if grad is not None:
+    grad = None
+    if want_grad:
         q_r = torch.exp(log_r - log_all)
         d = torch.where(rest, e.double() / s.double(), 0.0) * (q_r - p_r)
         d = torch.where(listed, el / norm - p, d) * (w * temperature)
         d = torch.where(live, d, 0.0)
         d = torch.where(bad, float("nan"), d)
         d = torch.where(skip | (z == -inf), 0.0, d)
-        _cpu_write(grad, d.to(grad.dtype), glay)
-    return loss.float().reshape(R)
+        grad = _cpu_write(logits, d, groups)
+    return loss.float().reshape(R), grad
 
 
 # ------------------------------------------------------------ dispatch
-def _compiled():
-    return torch.compiler.is_compiling()
+_compiled = torch.compiler.is_compiling
 
 
-def _grad_layout(shape, groups):
-    """(row stride, group offsets) of a contiguous tensor of the logits' shape."""
-    if groups is None:
-        return shape[-1], (0,)
-    return shape[1] * shape[2], _group_layout(groups, shape[2], shape[2])[0]
-
-
-def _run_log_probs(logits, mask, groups, targets, top_k, temperature, want_stats):
-    z, lay = _place(logits, groups)
-    m, ml = _place(mask, groups) if mask is not None else (None, lay)
-    if not z.is_cuda:
-        out = _cpu_log_probs(z, m if m is None else (m, ml), lay, targets, top_k, temperature)
-        lead = [lay.lead + (targets.shape[-1],), lay.lead, lay.lead, lay.lead + (top_k,),
-                lay.lead + (top_k,)]
-        return tuple(o.reshape(s) for o, s in zip(out, lead)) + (out[5],)
-    from . import ops
-    fn = ops.log_probs if _compiled() else ops.log_probs_impl
-    return fn(z, m, lay.lead, lay.n, lay.stride, lay.offsets, lay.sizes, ml.stride, ml.offsets,
-              targets, top_k, temperature, want_stats)
+def _run_log_probs(logits, mask, groups, lead, targets, top_k, temperature, want_stats):
+    if logits.is_cuda:
+        from . import ops
+        fn = ops.log_probs if _compiled() else ops.log_probs_impl
+        return fn(logits, mask, groups, targets, top_k, temperature, want_stats)
+    out = _cpu_log_probs(logits, mask, groups, targets, top_k, temperature)
+    shapes = (lead + (targets.shape[-1],), lead, lead, lead + (top_k,), lead + (top_k,))
+    return tuple(o.reshape(s) for o, s in zip(out, shapes)) + (out[5],)
 
 
 class _LogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, mask, groups, targets, top_k, temperature):
-        lp, h, norm, top, at, stats = _run_log_probs(logits, mask, groups, targets, top_k,
+    def forward(ctx, logits, mask, groups, lead, targets, top_k, temperature):
+        lp, h, norm, top, at, stats = _run_log_probs(logits, mask, groups, lead, targets, top_k,
                                                      temperature, True)
         ctx.save_for_backward(logits, mask, targets, at, stats, h)
         ctx.how = (groups, temperature)
@@ -350,20 +320,15 @@ class _LogProbs(torch.autograd.Function):
     def backward(ctx, g_lp, g_h, g_norm, g_top, _):
         logits, mask, targets, at, stats, h = ctx.saved_tensors
         groups, temperature = ctx.how
-        z, lay = _place(logits, groups)
-        m, ml = _place(mask, groups) if mask is not None else (None, lay)
-        gs = [None if g is None else g.contiguous() for g in (g_lp, g_h, g_norm, g_top)]
-        if z.is_cuda:
+        gs = [g if g is None or g.is_contiguous() else g.contiguous()
+              for g in (g_lp, g_h, g_norm, g_top)]
+        if not logits.is_cuda:
+            fn = _cpu_log_probs_backward
+        else:
             from . import ops
             fn = ops.log_probs_backward if _compiled() else ops.log_probs_backward_impl
-            grad = fn(z, m, logits.shape, lay.n, lay.stride, lay.offsets, lay.sizes, ml.stride,
-                      ml.offsets, *_grad_layout(logits.shape, groups), targets, at, stats, h, *gs,
-                      temperature)
-        else:
-            grad = torch.empty(logits.shape, dtype=logits.dtype)
-            _cpu_log_probs_backward(z, m if m is None else (m, ml), lay, targets, at, stats, h,
-                                    *gs, temperature, *_place(grad, groups))
-        return grad, None, None, None, None, None
+        grad = fn(logits, mask, groups, targets, at, stats, h, *gs, temperature)
+        return grad, None, None, None, None, None, None
 
 
 def profile_log_probs(logits, targets=None, *, top_k=0, mask=None, signal_groups=None,
@@ -381,85 +346,88 @@ def profile_log_probs(logits, targets=None, *, top_k=0, mask=None, signal_groups
     Returns ``ProfileLogProbs``; all but ``top_indices`` are differentiable
     with respect to the logits (once).
     """
-    groups, mask = _check(logits, mask, signal_groups, temperature)
+    groups, mask, lead = _check(logits, mask, signal_groups, temperature)
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= MAX_TOP:
         raise ValueError("top_k must be an int between 0 and {}, got {!r}".format(MAX_TOP, top_k))
-    lead = tuple(logits.shape[:-1]) if groups is None else (logits.shape[0], len(groups))
     if targets is None:
         targets = torch.empty(lead + (0,), dtype=torch.int64, device=logits.device)
     else:
-        targets = _check_list(targets, "targets", lead, logits.device, MAX_TARGETS)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return ProfileLogProbs(*_LogProbs.apply(logits, mask, groups, targets, top_k, temperature))
-    return ProfileLogProbs(*_run_log_probs(logits.detach(), mask, groups, targets, top_k,
+        targets = _check_list(targets, "targets", lead, logits.device)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return ProfileLogProbs(*_LogProbs.apply(logits, mask, groups, lead, targets, top_k,
+                                                temperature))
+    return ProfileLogProbs(*_run_log_probs(logits, mask, groups, lead, targets, top_k,
                                            temperature, False)[:5])
 
 
 # ------------------------------------------------------------ distillation
-def _run_distill(logits, mask, groups, idx, t_lp, renormalize, weight, scale, upstream, reduce,
-                 want_grad, temperature):
-    """(per-row losses, their sum or None, gradient or None)"""
-    z, lay = _place(logits, groups)
-    m, ml = _place(mask, groups) if mask is not None else (None, lay)
-    if not z.is_cuda:
-        grad = torch.empty(logits.shape, dtype=logits.dtype) if want_grad else None
-        rows = _cpu_distill(z, m if m is None else (m, ml), lay, idx, t_lp, renormalize, weight,
-                            scale, upstream, temperature,
-                            *(_place(grad, groups) if want_grad else (None, None)))
-        return rows.reshape(lay.lead), rows.double().sum().float() if reduce else None, grad
-    from . import ops
-    fn = ops.distill if _compiled() else ops.distill_impl
-    return fn(z, m, logits.shape, lay.lead, lay.n, lay.stride, lay.offsets, lay.sizes, ml.stride,
-              ml.offsets, *_grad_layout(logits.shape, groups), idx, t_lp, renormalize, weight,
-              scale, upstream, reduce, want_grad, temperature)
+def _run_distill(logits, mask, groups, lead, idx, t_lp, renormalize, weight, scale, upstream,
+                 want_losses, reduce, want_grad, temperature):
+    """(per-row losses, their sum, gradient: what is asked for)"""
+    if logits.is_cuda:
+        from . import ops
+        fn = ops.distill if _compiled() else ops.distill_impl
+        return fn(logits, mask, groups, idx, t_lp, renormalize, weight, scale, upstream,
+                  want_losses, reduce, want_grad, temperature)
+    rows, grad = _cpu_distill(logits, mask, groups, idx, t_lp, renormalize, weight, scale,
+                              upstream, want_grad, temperature)
+    return rows.reshape(lead), rows.double().sum().float() if reduce else None, grad
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, mask, groups, idx, t_lp, renormalize, weight, scale, reduce,
+    def forward(ctx, logits, mask, groups, lead, idx, t_lp, renormalize, weight, scale, reduce,
                 temperature):
-        rows, loss, _ = _run_distill(logits, mask, groups, idx, t_lp, renormalize, weight, scale,
-                                     None, reduce, False, temperature)
+        rows, loss, _ = _run_distill(logits, mask, groups, lead, idx, t_lp, renormalize, weight,
+                                     scale, None, not reduce, reduce, False, temperature)
         ctx.save_for_backward(logits, mask, idx, t_lp, weight)
-        ctx.how = (groups, renormalize, scale, temperature)
+        ctx.how = (groups, lead, renormalize, scale, temperature)
         return loss if reduce else rows
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         logits, mask, idx, t_lp, weight = ctx.saved_tensors
-        groups, renormalize, scale, temperature = ctx.how
-        _, _, grad = _run_distill(logits, mask, groups, idx, t_lp, renormalize, weight, scale,
-                                  g.contiguous(), False, True, temperature)
-        return (grad,) + (None,) * 9
+        groups, lead, renormalize, scale, temperature = ctx.how
+        if not g.is_contiguous():
+            g = g.contiguous()
+        grad = _run_distill(logits, mask, groups, lead, idx, t_lp, renormalize, weight, scale, g,
+                            False, False, True, temperature)[2]
+        return grad, None, None, None, None, None, None, None, None, None, None
 
 
 def _check_distill(logits, indices, log_probs, mask, signal_groups, temperature, weight,
                    reduction):
-    groups, mask = _check(logits, mask, signal_groups, temperature)
+    groups, mask, lead = _check(logits, mask, signal_groups, temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got {!r}".format(reduction))
-    lead = tuple(logits.shape[:-1]) if groups is None else (logits.shape[0], len(groups))
-    indices = _check_list(indices, "teacher_indices", lead, logits.device, MAX_TARGETS)
+    device = logits.device
+    indices = _check_list(indices, "teacher_indices", lead, device)
     if log_probs.shape != indices.shape or not log_probs.is_floating_point():
         _fail("teacher_log_probs must be floating and of teacher_indices' shape {}".format(
             tuple(indices.shape)))
+    if weight is not None and (weight.shape != lead or not weight.is_floating_point()):
+        _fail("weight must be floating and of shape {}, got {}".format(
+            lead, tuple(weight.shape)))
+    log_probs = _constant(log_probs, "teacher_log_probs", device)
     if weight is not None:
-        if tuple(weight.shape) != lead or not weight.is_floating_point():
-            _fail("weight must be floating and of shape {}, got {}".format(
-                lead, tuple(weight.shape)))
-    for t, name in ((log_probs, "teacher_log_probs"), (weight, "weight")):
-        if t is None:
-            continue
-        if t.device != logits.device:
-            _fail("{} must be on the logits' device".format(name))
-        if t.requires_grad and torch.is_grad_enabled():
-            _fail("{} takes no gradient: detach it".format(name))
-    log_probs = log_probs.detach().float().contiguous()
-    weight = weight.detach().float().contiguous() if weight is not None else None
-    rows = _numel(lead)
+        weight = _constant(weight, "weight", device)
+    rows = 1
+    for extent in lead:
+        rows *= extent
     scale = 1.0 / rows if reduction == "mean" and rows else 1.0
-    return groups, mask, indices, log_probs, weight, scale
+    return groups, mask, lead, indices, log_probs, weight, scale
+
+
+def _constant(t, name, device):
+    """t in fp32 and contiguous; it carries no gradient."""
+    if t.device != device:
+        _fail("{} must be on the logits' device".format(name))
+    if t.requires_grad:
+        if torch.is_grad_enabled():
+            _fail("{} takes no gradient: detach it".format(name))
+        t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def distillation_loss(logits, teacher_indices, teacher_log_probs, *, renormalize=False, mask=None,
@@ -486,18 +454,16 @@ def distillation_loss(logits, teacher_indices, teacher_log_probs, *, renormalize
     reduction: 'mean' over all rows, 'sum', or 'none' (lead). The result is
     fp32 and differentiable with respect to the logits (once).
     """
-    groups, mask, idx, t_lp, weight, scale = _check_distill(
+    groups, mask, lead, idx, t_lp, weight, scale = _check_distill(
         logits, teacher_indices, teacher_log_probs, mask, signal_groups, temperature, weight,
         reduction)
-    reduce = reduction != "none"
-    if torch.is_grad_enabled() and logits.requires_grad:
-        out = _Distill.apply(logits, mask, groups, idx, t_lp, bool(renormalize), weight, scale,
-                             reduce, temperature)
-    else:
-        rows, loss, _ = _run_distill(logits.detach(), mask, groups, idx, t_lp, bool(renormalize),
-                                     weight, scale, None, reduce, False, temperature)
-        out = loss if reduce else rows
-    return out
+    reduce, renormalize = reduction != "none", bool(renormalize)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Distill.apply(logits, mask, groups, lead, idx, t_lp, renormalize, weight, scale,
+                              reduce, temperature)
+    rows, loss, _ = _run_distill(logits, mask, groups, lead, idx, t_lp, renormalize, weight, scale,
+                                 None, not reduce, reduce, False, temperature)
+    return loss if reduce else rows
 
 
 def distillation_loss_and_grad(logits, teacher_indices, teacher_log_probs, *, renormalize=False,
@@ -510,10 +476,10 @@ def distillation_loss_and_grad(logits, teacher_indices, teacher_log_probs, *, re
     that of the losses' sum. Neither carries an autograd graph: continue with
     ``logits.backward(grad)``. What multiplies the loss goes into ``weight``.
     """
-    groups, mask, idx, t_lp, weight, scale = _check_distill(
+    groups, mask, lead, idx, t_lp, weight, scale = _check_distill(
         logits, teacher_indices, teacher_log_probs, mask, signal_groups, temperature, weight,
         reduction)
     reduce = reduction != "none"
-    rows, loss, grad = _run_distill(logits.detach(), mask, groups, idx, t_lp, bool(renormalize),
-                                    weight, scale, None, reduce, True, temperature)
+    rows, loss, grad = _run_distill(logits, mask, groups, lead, idx, t_lp, bool(renormalize),
+                                    weight, scale, None, not reduce, reduce, True, temperature)
     return (loss if reduce else rows), grad

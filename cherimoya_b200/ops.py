@@ -403,100 +403,164 @@ def _block_forward_fake(x, packed, packed_offset, hidden, dilation):
 
 
 # ----------------------------------------------------------------- likelihood, distillation
-# Rows are given as (z, lead, n, stride, offsets, sizes): n examples `stride`
-# elements apart, group g's first entry at offsets[g] and sizes[g] entries long
-# (chm_rows); `lead` is the shape of the per-row results. The functions named
-# *_impl are the bodies of the custom ops of the same name: eager callers call
-# them directly and save the dispatcher's share of a small call.
+# `groups` are the signal groups, empty where the last axis is a row. The
+# functions named *_impl are the bodies of the custom ops of the same name:
+# eager callers call them directly and save the dispatcher's share of a small
+# call, and get None for what they do not ask for.
 _LOGITS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-@functools.lru_cache(maxsize=256)
-def _host_array(kind, values):
-    return (kind * len(values))(*values)
+class RowPlan:
+    """Where the rows of a tensor of one shape and stride are, as chm_rows has them.
+
+    lead: shape of the per-row results; n examples `stride` elements apart;
+    group g's first entry at offsets[g], sizes[g] entries. None of it fits a
+    tensor that needs_copy: make that contiguous first."""
+
+    def __init__(self, shape, strides, groups):
+        width = shape[-1]
+        if groups:
+            self.lead = (shape[0], len(groups))
+            self.n, self.stride = shape[0], strides[0]
+            channel = strides[1]
+            self.needs_copy = (width > 1 and strides[2] != 1) or not (
+                channel == width or all(g == 1 for g in groups))
+            firsts = [sum(groups[:g]) for g in range(len(groups))]
+            self.offsets = tuple(f * channel for f in firsts)
+            self.sizes = tuple(g * width for g in groups)
+            self.grad_stride = shape[1] * width
+            self.grad_offsets = tuple(f * width for f in firsts)
+        else:
+            self.lead = shape[:-1]
+            self.n = 1
+            for extent in self.lead:
+                self.n *= extent
+            # one stride must lead from row to row
+            self.stride, self.needs_copy = width, width > 1 and strides[-1] != 1
+            axes = [(e, t) for e, t in zip(self.lead, strides) if e != 1]
+            if axes:
+                self.stride = axes[-1][1]
+                self.needs_copy |= any(a[1] != b[0] * b[1] for a, b in zip(axes, axes[1:]))
+            self.offsets, self.sizes = (0,), (width,)
+            self.grad_stride, self.grad_offsets = width, (0,)
+        self.rows = self.n * len(self.sizes)
+        self._arrays = ((ctypes.c_int64 * len(self.sizes))(*self.offsets),
+                        (ctypes.c_int32 * len(self.sizes))(*self.sizes),
+                        (ctypes.c_int64 * len(self.sizes))(*self.grad_offsets))
+        self.at = tuple(ctypes.addressof(a) for a in self._arrays)
 
 
-def _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets, grad, grad_stride,
-                 grad_offsets, temperature):
-    keep = (_host_array(ctypes.c_int64, tuple(offsets)), _host_array(ctypes.c_int32, tuple(sizes)),
-            _host_array(ctypes.c_int64, tuple(mask_offsets)) if mask is not None else None,
-            _host_array(ctypes.c_int64, tuple(grad_offsets)) if grad is not None else None)
-    at = [ctypes.addressof(k) if k is not None else None for k in keep]
-    rows = _lib.Rows(z.data_ptr(), _LOGITS[z.dtype], len(sizes), n, stride, at[0], at[1],
-                     _addr(mask), mask_stride, at[2], _addr(grad), grad_stride, at[3], temperature)
-    rows.keep = keep               # the struct holds bare addresses
-    return rows
+@functools.lru_cache(maxsize=1024)
+def row_plan(shape, strides, groups):
+    return RowPlan(shape, strides, groups)
+
+
+def place_rows(x, groups):
+    """(x, or a contiguous copy of it; its plan)"""
+    plan = row_plan(x.shape, x.stride(), groups)
+    if plan.needs_copy:
+        x = x.contiguous()
+        plan = row_plan(x.shape, x.stride(), groups)
+    return x, plan
+
+
+def _rows_struct(z, plan, mask, mask_plan, grad, temperature):
+    """chm_rows; the plans own what it points to on the host."""
+    return _lib.Rows(
+        z.data_ptr(), _LOGITS[z.dtype], len(plan.sizes), plan.n, plan.stride, plan.at[0],
+        plan.at[1], None if mask is None else mask.data_ptr(),
+        0 if mask is None else mask_plan.stride, None if mask is None else mask_plan.at[0],
+        None if grad is None else grad.data_ptr(), plan.grad_stride, plan.at[2], temperature)
 
 
 def _on(device, fn, *args):
     """fn(*args, stream) with `device` current."""
-    if torch.cuda.current_device() == device.index:
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _addr(t):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
-def log_probs_impl(z: torch.Tensor, mask: Optional[torch.Tensor], lead: List[int], n: int,
-                   stride: int, offsets: List[int], sizes: List[int], mask_stride: int,
-                   mask_offsets: List[int], targets: torch.Tensor, top_k: int, temperature: float,
-                   want_stats: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor,
-                                              torch.Tensor, torch.Tensor, torch.Tensor]:
+def log_probs_impl(logits: torch.Tensor, mask: Optional[torch.Tensor], groups: List[int],
+                   targets: torch.Tensor, top_k: int, temperature: float, want_stats: bool
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                              torch.Tensor, torch.Tensor]:
     """Log probabilities of targets, entropy, log normaliser, top log
     probabilities, top indices, and the statistics log_probs_backward reads."""
     lib = _lib.load()
-    _require_cuda(z, "logits")
-    S, dev, lead = targets.shape[-1], z.device, tuple(lead)
-    lp = torch.empty(lead + (S,), dtype=torch.float32, device=dev)
-    h = torch.empty(lead, dtype=torch.float32, device=dev)
-    norm = torch.empty(lead, dtype=torch.float32, device=dev)
-    top = torch.empty(lead + (top_k,), dtype=torch.float32, device=dev)
-    at = torch.empty(lead + (top_k,), dtype=torch.int64, device=dev)
-    stats = torch.empty((n * len(sizes) if want_stats else 0, 2), dtype=torch.float32, device=dev)
-    rows = _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets, None, 0,
-                        (), temperature)
-    st = _on(dev, lib.chm_log_probs, rows, targets.data_ptr(), S, top_k, lp.data_ptr(),
-             h.data_ptr(), norm.data_ptr(), top.data_ptr(), at.data_ptr(),
-             stats.data_ptr() if want_stats else None)
+    _require_cuda(logits, "logits")
+    groups = tuple(groups)
+    z, plan = place_rows(logits, groups)
+    mask, mask_plan = (None, None) if mask is None else place_rows(mask, groups)
+    f32, dev, lead = torch.float32, z.device, plan.lead
+    S = targets.shape[-1]
+    lp = torch.empty(*lead, S, dtype=f32, device=dev)
+    h = torch.empty(lead, dtype=f32, device=dev)
+    norm = torch.empty_like(h)
+    top = torch.empty(*lead, top_k, dtype=f32, device=dev)
+    at = torch.empty(*lead, top_k, dtype=torch.int64, device=dev)
+    stats = torch.empty(plan.rows, 2, dtype=f32, device=dev) if want_stats else None
+    st = _on(dev, lib.chm_log_probs, _rows_struct(z, plan, mask, mask_plan, None, temperature),
+             targets.data_ptr(), S, top_k, lp.data_ptr(), h.data_ptr(), norm.data_ptr(),
+             top.data_ptr(), at.data_ptr(), stats.data_ptr() if want_stats else None)
     _lib.check(st, "log_probs")
     return lp, h, norm, top, at, stats
 
 
-log_probs = torch.library.custom_op("cherimoya_b200::log_probs", log_probs_impl, mutates_args=())
+def _log_probs_op(logits: torch.Tensor, mask: Optional[torch.Tensor], groups: List[int],
+                  targets: torch.Tensor, top_k: int, temperature: float, want_stats: bool
+                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                             torch.Tensor, torch.Tensor]:
+    out = log_probs_impl(logits, mask, groups, targets, top_k, temperature, want_stats)
+    return out if want_stats else out[:5] + (out[0].new_empty((0, 2)),)
+
+
+log_probs = torch.library.custom_op("cherimoya_b200::log_probs", _log_probs_op, mutates_args=())
+
+
+def _lead(logits, groups):
+    return (logits.shape[0], len(groups)) if len(groups) else tuple(logits.shape[:-1])
 
 
 @log_probs.register_fake
-def _log_probs_fake(z, mask, lead, n, stride, offsets, sizes, mask_stride, mask_offsets, targets,
-                    top_k, temperature, want_stats):
+def _log_probs_fake(logits, mask, groups, targets, top_k, temperature, want_stats):
+    lead = _lead(logits, groups)
+    rows = 1
+    for extent in lead:
+        rows = rows * extent
+
     def f32(*shape):
-        return z.new_empty(shape, dtype=torch.float32)
+        return logits.new_empty(shape, dtype=torch.float32)
     return (f32(*lead, targets.shape[-1]), f32(*lead), f32(*lead), f32(*lead, top_k),
-            z.new_empty((*lead, top_k), dtype=torch.int64),
-            f32(n * len(sizes) if want_stats else 0, 2))
+            logits.new_empty((*lead, top_k), dtype=torch.int64),
+            f32(rows if want_stats else 0, 2))
 
 
-def log_probs_backward_impl(z: torch.Tensor, mask: Optional[torch.Tensor], shape: List[int],
-                            n: int, stride: int, offsets: List[int], sizes: List[int],
-                            mask_stride: int, mask_offsets: List[int], grad_stride: int,
-                            grad_offsets: List[int], targets: torch.Tensor,
-                            top_indices: torch.Tensor, stats: torch.Tensor,
-                            entropy: torch.Tensor, g_log_probs: Optional[torch.Tensor],
+def log_probs_backward_impl(logits: torch.Tensor, mask: Optional[torch.Tensor],
+                            groups: List[int], targets: torch.Tensor, top_indices: torch.Tensor,
+                            stats: torch.Tensor, entropy: torch.Tensor,
+                            g_log_probs: Optional[torch.Tensor],
                             g_entropy: Optional[torch.Tensor], g_norm: Optional[torch.Tensor],
                             g_top: Optional[torch.Tensor], temperature: float) -> torch.Tensor:
-    """Gradient of log_probs' outputs, a contiguous tensor of `shape`."""
+    """Gradient of log_probs' outputs: contiguous, of the logits' shape and type."""
     lib = _lib.load()
-    _require_cuda(z, "logits")
-    grad = torch.empty(tuple(shape), dtype=z.dtype, device=z.device)
-    if grad.numel() == 0:
+    _require_cuda(logits, "logits")
+    groups = tuple(groups)
+    z, plan = place_rows(logits, groups)
+    mask, mask_plan = (None, None) if mask is None else place_rows(mask, groups)
+    grad = torch.empty(logits.shape, dtype=z.dtype, device=z.device)
+    if plan.rows == 0 or grad.numel() == 0:
         return grad
-    rows = _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets, grad,
-                        grad_stride, grad_offsets, temperature)
-    st = _on(z.device, lib.chm_log_probs_backward, rows, targets.data_ptr(), targets.shape[-1],
-             top_indices.data_ptr(), top_indices.shape[-1], stats.data_ptr(), entropy.data_ptr(),
-             _addr(g_log_probs), _addr(g_entropy), _addr(g_norm), _addr(g_top))
+    st = _on(z.device, lib.chm_log_probs_backward,
+             _rows_struct(z, plan, mask, mask_plan, grad, temperature), targets.data_ptr(),
+             targets.shape[-1], top_indices.data_ptr(), top_indices.shape[-1], stats.data_ptr(),
+             entropy.data_ptr(), _addr(g_log_probs), _addr(g_entropy), _addr(g_norm),
+             _addr(g_top))
     _lib.check(st, "log_probs_backward")
     return grad
 
@@ -506,43 +570,54 @@ log_probs_backward = torch.library.custom_op("cherimoya_b200::log_probs_backward
 
 
 @log_probs_backward.register_fake
-def _log_probs_backward_fake(z, mask, shape, *rest):
-    return z.new_empty(shape)
+def _log_probs_backward_fake(logits, *rest):
+    return logits.new_empty(logits.shape)
 
 
-def distill_impl(z: torch.Tensor, mask: Optional[torch.Tensor], shape: List[int], lead: List[int],
-                 n: int, stride: int, offsets: List[int], sizes: List[int], mask_stride: int,
-                 mask_offsets: List[int], grad_stride: int, grad_offsets: List[int],
+def distill_impl(logits: torch.Tensor, mask: Optional[torch.Tensor], groups: List[int],
                  indices: torch.Tensor, log_probs: torch.Tensor, renormalize: bool,
                  weight: Optional[torch.Tensor], scale: float, upstream: Optional[torch.Tensor],
-                 reduce: bool, want_grad: bool,
-                 temperature: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Distillation losses of the rows, their sum (with `reduce`), and the
-    gradient (with `want_grad`, a contiguous tensor of `shape`); what is not
-    wanted is empty."""
+                 want_losses: bool, reduce: bool, want_grad: bool, temperature: float
+                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Distillation losses of the rows (with `want_losses`), their sum (with
+    `reduce`), and the gradient (with `want_grad`: contiguous, of the logits'
+    shape and type)."""
     lib = _lib.load()
-    _require_cuda(z, "logits")
+    _require_cuda(logits, "logits")
+    groups = tuple(groups)
+    z, plan = place_rows(logits, groups)
+    mask, mask_plan = (None, None) if mask is None else place_rows(mask, groups)
     dev = z.device
-    losses = torch.empty(tuple(lead), dtype=torch.float32, device=dev)
-    loss = torch.empty(() if reduce else (0,), dtype=torch.float32, device=dev)
-    grad = torch.empty(tuple(shape) if want_grad else (0,), dtype=z.dtype, device=dev)
-    rows = _rows_struct(z, mask, n, stride, offsets, sizes, mask_stride, mask_offsets,
-                        grad if want_grad else None, grad_stride, grad_offsets, temperature)
-    st = _on(dev, lib.chm_distill, rows, indices.data_ptr(), log_probs.data_ptr(),
-             indices.shape[-1], renormalize, _addr(weight), scale, _addr(upstream),
-             1 if upstream is not None and upstream.dim() > 0 else 0, losses.data_ptr(),
-             loss.data_ptr() if reduce else None)
+    losses = torch.empty(plan.lead, dtype=torch.float32, device=dev) \
+        if want_losses or reduce else None
+    loss = torch.empty((), dtype=torch.float32, device=dev) if reduce else None
+    grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if want_grad else None
+    st = _on(dev, lib.chm_distill, _rows_struct(z, plan, mask, mask_plan, grad, temperature),
+             indices.data_ptr(), log_probs.data_ptr(), indices.shape[-1], renormalize,
+             _addr(weight), scale, _addr(upstream),
+             1 if upstream is not None and upstream.dim() > 0 else 0, _addr(losses),
+             _addr(loss))
     _lib.check(st, "distill")
     return losses, loss, grad
 
 
-distill = torch.library.custom_op("cherimoya_b200::distill", distill_impl, mutates_args=())
+def _distill_op(logits: torch.Tensor, mask: Optional[torch.Tensor], groups: List[int],
+                indices: torch.Tensor, log_probs: torch.Tensor, renormalize: bool,
+                weight: Optional[torch.Tensor], scale: float, upstream: Optional[torch.Tensor],
+                want_losses: bool, reduce: bool, want_grad: bool, temperature: float
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    out = distill_impl(logits, mask, groups, indices, log_probs, renormalize, weight, scale,
+                       upstream, True, reduce, want_grad, temperature)
+    return (out[0], out[1] if reduce else out[0].new_empty((0,)),
+            out[2] if want_grad else logits.new_empty((0,)))
+
+
+distill = torch.library.custom_op("cherimoya_b200::distill", _distill_op, mutates_args=())
 
 
 @distill.register_fake
-def _distill_fake(z, mask, shape, lead, n, stride, offsets, sizes, mask_stride, mask_offsets,
-                  grad_stride, grad_offsets, indices, log_probs, renormalize, weight, scale,
-                  upstream, reduce, want_grad, temperature):
-    return (z.new_empty(lead, dtype=torch.float32),
-            z.new_empty(() if reduce else (0,), dtype=torch.float32),
-            z.new_empty(shape if want_grad else (0,)))
+def _distill_fake(logits, mask, groups, indices, log_probs, renormalize, weight, scale, upstream,
+                  want_losses, reduce, want_grad, temperature):
+    return (logits.new_empty(_lead(logits, groups), dtype=torch.float32),
+            logits.new_empty(() if reduce else (0,), dtype=torch.float32),
+            logits.new_empty(logits.shape if want_grad else (0,)))
