@@ -1121,13 +1121,13 @@ static __device__ __noinline__ double exp64(double x) { return exp(x); }
 // Per warp: what the list adds up to.
 struct ListSums {
   double mass, p_log_p, p_z;       // sum P, P log P, P z'
-  float e;                         // sum exp(z')
+  double e;                        // sum exp(z')
   float top_z, top_lp;             // the warp's largest z, log P: z' and P are relative to them
 };
 // What a warp's part of the list adds up to; p becomes P from log P.
 template <int kThreads>
 __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int* idx, int K,
-                                           int renormalize, float inv_t) {
+                                           int renormalize, double inv_t) {
   float top_lp = neg_inf(), top_z = neg_inf();
 #pragma unroll 1
   for (int k = Team<kThreads>::tid(); k < K; k += kThreads)
@@ -1141,19 +1141,19 @@ __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int
     top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
   }
   if (!renormalize || top_lp == neg_inf()) top_lp = 0.f;
-  ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
+  ListSums ls{0.0, 0.0, 0.0, 0.0, top_z, top_lp};
 #pragma unroll 1
   for (int k = Team<kThreads>::tid(); k < K; k += kThreads) {
     if (idx[k] < 0) continue;
     const double lp = p[k] - (double)top_lp, pk = exp64(lp);
-    const float zp = (zu[k] - top_z) * inv_t;
+    const double zp = ((double)zu[k] - (double)top_z) * inv_t;
     p[k] = pk;
     ls.mass += pk;
     if (pk > 0.0) {
       ls.p_log_p += pk * lp;
-      ls.p_z += pk * (double)zp;
+      ls.p_z += pk * zp;
     }
-    ls.e += expf(zp);
+    ls.e += exp64(zp);
   }
 #pragma unroll 1
   for (int w = 16; w > 0; w >>= 1) {
@@ -1168,26 +1168,27 @@ __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int
 // The warps' parts of the list, relative to the largest z and log P of all, as
 // the first one's; factor: of each warp's P to the common ones. One warp.
 template <int kThreads>
-__device__ __noinline__ void join_list(ListSums* part, float* factor, int warps, float inv_t) {
+__device__ __noinline__ void join_list(ListSums* part, float* factor, int warps, double inv_t) {
   float top_z = neg_inf(), top_lp = neg_inf();
   for (int w = 0; w < warps; ++w) {
     top_z = fmaxf(top_z, part[w].top_z);
     if (part[w].mass > 0.0) top_lp = fmaxf(top_lp, part[w].top_lp);
   }
-  ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
+  ListSums ls{0.0, 0.0, 0.0, 0.0, top_z, top_lp};
 #pragma unroll 1
   for (int w = 0; w < warps; ++w) {
     const ListSums b = part[w];
     const double up = b.mass > 0.0 ? (double)b.top_lp - (double)top_lp : 0.0;
     const double f = up == 0.0 ? 1.0 : exp64(up);
-    const float zp = b.top_z == neg_inf() ? 0.f : (b.top_z - top_z) * inv_t;
+    const double zp =
+        b.top_z == neg_inf() ? 0.0 : ((double)b.top_z - (double)top_z) * inv_t;
     if (Team<kThreads>::lane() == 0) factor[w] = (float)f;
     ls.mass += f * b.mass;
     if (b.mass > 0.0) {
       ls.p_log_p += f * (b.p_log_p + up * b.mass);
-      ls.p_z += f * (b.p_z + (double)zp * b.mass);
+      ls.p_z += f * (b.p_z + zp * b.mass);
     }
-    ls.e += b.e * (zp == 0.f ? 1.f : expf(zp));
+    ls.e += b.e * (zp == 0.0 ? 1.0 : exp64(zp));
   }
   __syncwarp();
   if (warps > 0 && Team<kThreads>::lane() == 0) part[0] = ls;
@@ -1261,6 +1262,9 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   const Share<T> share(row, rank, log_blocks, Tm::tid());
   unsigned char* mine = dyn + slot * team_bytes;
   const uint32_t chunk = smem_u32(mine);
+  // 1 / T as the exponentials have it: rounded with log2(e) in a.c, the same everywhere, so that
+  // loss and gradient are those of one temperature, off by half a step of fp32
+  const double inv_t = (double)a.c * 0.69314718055994531;
   double* p = reinterpret_cast<double*>(mine + chunks * cap * 16);
   float* zu = reinterpret_cast<float*>(p + K);
   int* idx = reinterpret_cast<int*>(zu + K);
@@ -1320,7 +1324,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     }
     const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (again ? 2u : 0u));
     if (Tm::lane() == 0) flags[slot][Tm::warp()] = flag;
-    const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, a.inv_t);
+    const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, inv_t);
     if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
   }
   // the rest of the row
@@ -1345,9 +1349,9 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
       const int v = idx[k];
       if (v >= first && v < last) sts_neg_inf<T>(now + (v - first) * (int)sizeof(T));
     }
-    if (base == share.begin && Tm::warp() == Tm::kWarps - 1)
-      join_list<kThreads>(lred[slot], factor[slot], list_warps, a.inv_t);
     Tm::sync();
+    if (base == share.begin && Tm::warp() == Tm::kWarps - 1)   // wanted after the sums
+      join_list<kThreads>(lred[slot], factor[slot], list_warps, inv_t);
     uint32_t at = now + Tm::tid() * 16;
 #pragma unroll 1
     for (int i = 0; i < n; i += kBatch) {
@@ -1382,11 +1386,11 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     Tm::sync();
     merge_list<kThreads>(p, idx, K);
     if (Tm::warp() < list_warps) {
-      const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, a.inv_t);
+      const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, inv_t);
       if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
     }
     Tm::sync();
-    if (Tm::warp() == 0) join_list<kThreads>(lred[slot], factor[slot], list_warps, a.inv_t);
+    if (Tm::warp() == 0) join_list<kThreads>(lred[slot], factor[slot], list_warps, inv_t);
     Tm::sync();
   }
   sum = team_sums<kThreads>(sum, a.c, red[slot]);   // orders lred, too (a barrier, or one warp)
@@ -1403,7 +1407,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
 #pragma unroll 1
     for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
   }
-  const ListSums ls = K > 0 ? lred[slot][0] : ListSums{0.0, 0.0, 0.0, 0.f, neg_inf(), 0.f};
+  const ListSums ls = K > 0 ? lred[slot][0] : ListSums{0.0, 0.0, 0.0, 0.0, neg_inf(), 0.f};
   const bool rest = sum.m != neg_inf(), listed = ls.top_z != neg_inf();
   bad = (all & 1) || sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
   const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
@@ -1412,22 +1416,31 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
   // the two normalisers relative to the larger of the two maxima
   const float big = fmaxf(rest ? sum.m : neg_inf(), ls.top_z);
-  const float down_r = rest ? (sum.m - big) * a.inv_t : 0.f;
-  const float down_u = listed ? (ls.top_z - big) * a.inv_t : 0.f;
-  const float norm_r = rest ? sum.s * expf(down_r) : 0.f;
-  const float norm = norm_r + (listed ? ls.e * expf(down_u) : 0.f);
-  auto write_loss = [&]() {                       // by one thread, when the others are done
-    if (rank != 0 || Tm::tid() != kThreads - 1 || !o.row_loss) return;
-    const double log_all = logf(norm);
+  const float norm_r = rest ? sum.s * ex2((sum.m - big) * a.c) : 0.f;
+  const float norm = norm_r + (listed ? (float)ls.e * ex2((ls.top_z - big) * a.c) : 0.f);
+  // by the last warp, when the others are done; a function call to a lane
+  auto write_loss = [&]() {
+    if (rank != 0 || Tm::warp() != Tm::kWarps - 1 || !o.row_loss) return;
+    const int lane = Tm::lane();
+    const double down_r = rest ? ((double)sum.m - (double)big) * inv_t : 0.0;
+    const double down_u = listed ? ((double)ls.top_z - (double)big) * inv_t : 0.0;
+    const double rest_mass = whole ? 0.0 : 1.0 - ls.mass;
+    double e = exp64(lane == 0 ? down_r : down_u);          // 0: the rest, 1: the list
+    e *= lane == 0 ? (rest ? (double)sum.s : 0.0) : (listed ? ls.e : 0.0);
+    const double norm64 = __shfl_sync(0xffffffffu, e, 0) + __shfl_sync(0xffffffffu, e, 1);
+    const double l = log(lane == 0 ? norm64 : lane == 1 ? ls.mass : lane == 2 ? rest_mass
+                                                                              : (double)sum.s);
+    const double log_all = __shfl_sync(0xffffffffu, l, 0), log_mass = __shfl_sync(0xffffffffu, l, 1);
+    const double log_p_r = __shfl_sync(0xffffffffu, l, 2), log_s = __shfl_sync(0xffffffffu, l, 3);
     double loss = 0.0;
     if (live && ls.mass > 0.0) {
-      loss = ls.p_log_p - ls.p_z + (log_all - (double)down_u) * ls.mass;
-      if (whole) loss = loss / ls.mass - log(ls.mass);
+      loss = ls.p_log_p - ls.p_z + (log_all - down_u) * ls.mass;
+      if (whole) loss = loss / ls.mass - log_mass;
     }
-    if (live && p_r > 0.f)
-      loss += (double)p_r * ((double)logf(p_r) - ((double)down_r + (double)logf(sum.s) - log_all));
-    o.row_loss[row.index] =
-        bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
+    if (live && rest_mass > 0.0) loss += rest_mass * (log_p_r - (down_r + log_s - log_all));
+    if (lane == 0)
+      o.row_loss[row.index] =
+          bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
   };
   if (!row.grad) {
     write_loss();
