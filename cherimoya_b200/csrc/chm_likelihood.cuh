@@ -231,8 +231,11 @@ struct Row {
   __device__ __forceinline__ bool vec_store() const {
     return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
   }
+  // entry v; the mask's byte and the logit are asked for together
   __device__ __forceinline__ float at(int v) const {
-    return (mask && !mask[v]) ? neg_inf() : to_float(z[v]);
+    const uint8_t in = mask ? mask[v] : 1;
+    const float f = to_float(z[v]);
+    return in ? f : neg_inf();
   }
   __device__ __forceinline__ const T* vec(int j) const { return z + head + (long long)j * N; }
   // the mask's bytes for vector j
@@ -1116,21 +1119,37 @@ template <typename T> __device__ __forceinline__ void sts_neg_inf(uint32_t a) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((uint16_t)Vec<T>::kNegInf) : "memory");
 }
 
-static __device__ __noinline__ double exp64(double x) { return exp(x); }
+// exp in 64 bits, for masses that are added up and taken from 1: x = n log 2 + r
+// with |r| <= log(2) / 2, and the Taylor sum of e^r to r^11 (the rest is below
+// 7e-15) in a tree, since one call after the other waits for fp64's latency.
+// 0 below -700, where no mass is left; inf above 700.
+__device__ __forceinline__ double exp64(double x) {
+  const double n = rint(x * 1.4426950408889634);
+  const double r = fma(n, -1.9082149292705877e-10, fma(n, -6.9314718036912382e-1, x));
+  const double r2 = r * r, r4 = r2 * r2;
+  const double a = fma(fma(1.0 / 6, r, 0.5), r2, 1.0 + r);
+  const double b = fma(fma(1.0 / 5040, r, 1.0 / 720), r2, fma(1.0 / 120, r, 1.0 / 24));
+  const double c = fma(fma(1.0 / 39916800, r, 1.0 / 3628800), r2,
+                       fma(1.0 / 362880, r, 1.0 / 40320));
+  const double e = fma(fma(c, r4, b), r4, a);
+  const int k = (int)fmin(fmax(n, -1010.0), 1010.0);
+  const double s = e * __hiloint2double((1023 + k) << 20, 0);
+  return x < -700.0 ? 0.0 : x > 700.0 ? (double)__int_as_float(0x7f800000) : s;
+}
 
 // Per warp: what the list adds up to.
 struct ListSums {
   double mass, p_log_p, p_z;       // sum P, P log P, P z'
-  double e;                        // sum exp(z')
+  float e;                         // sum exp(z')
   float top_z, top_lp;             // the warp's largest z, log P: z' and P are relative to them
 };
-// What a warp's part of the list adds up to; p becomes P from log P.
-template <int kThreads>
-__device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int* idx, int K,
-                                           int renormalize, double inv_t) {
+// What a warp's part of the list (entries first, first + step, ... of its lanes)
+// adds up to; p becomes P from log P.
+static __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int* idx, int K,
+                                           int first, int step, int renormalize, double inv_t) {
   float top_lp = neg_inf(), top_z = neg_inf();
 #pragma unroll 1
-  for (int k = Team<kThreads>::tid(); k < K; k += kThreads)
+  for (int k = first; k < K; k += step)
     if (idx[k] >= 0) {
       top_lp = fmaxf(top_lp, (float)p[k]);
       top_z = fmaxf(top_z, zu[k]);
@@ -1141,9 +1160,9 @@ __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int
     top_z = fmaxf(top_z, __shfl_xor_sync(0xffffffffu, top_z, w));
   }
   if (!renormalize || top_lp == neg_inf()) top_lp = 0.f;
-  ListSums ls{0.0, 0.0, 0.0, 0.0, top_z, top_lp};
+  ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
 #pragma unroll 1
-  for (int k = Team<kThreads>::tid(); k < K; k += kThreads) {
+  for (int k = first; k < K; k += step) {
     if (idx[k] < 0) continue;
     const double lp = p[k] - (double)top_lp, pk = exp64(lp);
     const double zp = ((double)zu[k] - (double)top_z) * inv_t;
@@ -1153,7 +1172,7 @@ __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int
       ls.p_log_p += pk * lp;
       ls.p_z += pk * zp;
     }
-    ls.e += exp64(zp);
+    ls.e += expf((float)zp);
   }
 #pragma unroll 1
   for (int w = 16; w > 0; w >>= 1) {
@@ -1165,16 +1184,16 @@ __device__ __noinline__ ListSums list_sums(double* p, const float* zu, const int
   return ls;
 }
 
-// The warps' parts of the list, relative to the largest z and log P of all, as
-// the first one's; factor: of each warp's P to the common ones. One warp.
-template <int kThreads>
-__device__ __noinline__ void join_list(ListSums* part, float* factor, int warps, double inv_t) {
+// The warps' parts of the list, relative to the largest z and log P of all;
+// factor: of warp `mine`'s P to the common ones.
+static __device__ __noinline__ ListSums join_list(const ListSums* part, int warps, int mine, double inv_t,
+                                           float* factor) {
   float top_z = neg_inf(), top_lp = neg_inf();
   for (int w = 0; w < warps; ++w) {
     top_z = fmaxf(top_z, part[w].top_z);
     if (part[w].mass > 0.0) top_lp = fmaxf(top_lp, part[w].top_lp);
   }
-  ListSums ls{0.0, 0.0, 0.0, 0.0, top_z, top_lp};
+  ListSums ls{0.0, 0.0, 0.0, 0.f, top_z, top_lp};
 #pragma unroll 1
   for (int w = 0; w < warps; ++w) {
     const ListSums b = part[w];
@@ -1182,16 +1201,15 @@ __device__ __noinline__ void join_list(ListSums* part, float* factor, int warps,
     const double f = up == 0.0 ? 1.0 : exp64(up);
     const double zp =
         b.top_z == neg_inf() ? 0.0 : ((double)b.top_z - (double)top_z) * inv_t;
-    if (Team<kThreads>::lane() == 0) factor[w] = (float)f;
+    if (w == mine) *factor = (float)f;
     ls.mass += f * b.mass;
     if (b.mass > 0.0) {
       ls.p_log_p += f * (b.p_log_p + up * b.mass);
       ls.p_z += f * (b.p_z + zp * b.mass);
     }
-    ls.e += b.e * (zp == 0.0 ? 1.0 : exp64(zp));
+    ls.e += b.e * expf((float)zp);
   }
-  __syncwarp();
-  if (warps > 0 && Team<kThreads>::lane() == 0) part[0] = ls;
+  return ls;
 }
 
 // A list in which an entry may be twice: the first one takes the others' mass
@@ -1239,6 +1257,7 @@ __device__ __noinline__ void merge_list(double* p, int* idx, int K) {
 //   dz_u = T w (exp(z'_u - lse) - P_u)              in it
 // so the gradient is one more exponential per entry in shared memory. Without
 // a gradient the chunks are small and there are two, one on its way.
+// The first warps add up the list while the others begin with the row.
 // At least three blocks of 256 to an SM, which 64 KB of shared memory allow.
 template <typename T, int kThreads, bool kMask>
 __global__ void
@@ -1250,7 +1269,6 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Sums red[Tm::kPerBlock][Tm::kWarps];
   __shared__ ListSums lred[Tm::kPerBlock][Tm::kWarps];
-  __shared__ float factor[Tm::kPerBlock][Tm::kWarps];   // of a warp's p, to that of all
   __shared__ int flags[Tm::kPerBlock][Tm::kWarps];
   __shared__ float cl[kMaxCluster][2];            // every block's maximum and sum
   const int slot = Tm::slot(), K = o.n_listed;
@@ -1258,8 +1276,6 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   const unsigned r0 = (blockIdx.x >> log_blocks) * Tm::kPerBlock + slot;
   if (kThreads == 32 && r0 >= rows) return;
   if (blocks > 1) cluster_arrive();
-  const Row<T> row(a, r0);
-  const Share<T> share(row, rank, log_blocks, Tm::tid());
   unsigned char* mine = dyn + slot * team_bytes;
   const uint32_t chunk = smem_u32(mine);
   // 1 / T as the exponentials have it: rounded with log2(e) in a.c, the same everywhere, so that
@@ -1269,8 +1285,13 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   float* zu = reinterpret_cast<float*>(p + K);
   int* idx = reinterpret_cast<int*>(zu + K);
   uint32_t* seen = reinterpret_cast<uint32_t*>(idx + K);
+  const int load_warps = min(Tm::kWarps, (K + 31) / 32);    // they have entries to load
+  // they add the list up: a power of two, about 128 entries to each
+  const int list_warps = K == 0 ? 0 : min(Tm::kWarps, K <= 128 ? 1 : 1 << (32 - __clz((K - 1) / 128)));
+  const Row<T> row(a, r0);
+  const Share<T> share(row, rank, log_blocks, Tm::tid());
   const bool one = share.end - share.begin <= cap, vec_store = row.vec_store();
-  float weight = o.weight ? o.weight[row.index] : 1.f;
+  const float weight = o.weight ? o.weight[row.index] : 1.f;
   copy_chunk<T, kThreads>(chunk, row, share.begin,
                           own_vectors<kThreads>(share.begin, min(share.begin + cap, share.end)));
   if (weight == 0.f) {                            // nothing of the row is looked at
@@ -1287,12 +1308,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     if (blocks > 1) cluster_wait();
     return;
   }
-  weight *= o.scale;
-  if (o.upstream) weight *= o.upstream[row.index * o.upstream_stride];
-  const int words = seen_words(row.size);
-  for (int w = Tm::tid(); w < words; w += kThreads) seen[w] = 0u;
-  const int list_warps = min(Tm::kWarps, (K + 31) / 32);   // the warps that hold some of the list
-  bool bad = false;
+  uint32_t flag = 0;              // 1: a bad entry of the list; 2: one there twice, or so it seems
   // While the row is on its way: the list, an entry to a thread.
 #pragma unroll 1
   for (int k = Tm::tid(); k < K; k += kThreads) {
@@ -1300,11 +1316,13 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     const float lp = o.log_probs[row.index * K + k];
     const float z = i >= 0 && i < row.size ? row.at((int)i) : neg_inf();
     const bool there = z != neg_inf();
-    bad |= i >= row.size || (there && !(lp < -neg_inf()));
+    if (i >= row.size || (there && !(lp < -neg_inf()))) flag = 1u;
     idx[k] = there ? (int)i : -1;
     zu[k] = z;
     p[k] = (double)lp;
   }
+  const int words = seen_words(row.size);
+  for (int w = Tm::tid(); w < words; w += kThreads) seen[w] = 0u;
   typename Row<T>::MaskBytes ahead[kBatch];       // the first batch's mask
   auto fetch_mask = [&](int base, int i, int n) {
 #pragma unroll
@@ -1315,24 +1333,22 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     fetch_mask(share.begin, 0,
                own_vectors<kThreads>(share.begin, min(share.begin + cap, share.end)));
   Tm::sync();                                     // the marks are clear
-  if (Tm::warp() < list_warps) {
-    bool again = false;                           // is an entry there twice? (or seems to be)
+  if (Tm::warp() < load_warps) {
 #pragma unroll 1
     for (int k = Tm::tid(); k < K; k += kThreads) {
       const int v = idx[k] & (kSeenBits - 1);
-      if (idx[k] >= 0) again |= (atomicOr(&seen[v >> 5], 1u << (v & 31)) >> (v & 31)) & 1u;
+      if (idx[k] >= 0 && ((atomicOr(&seen[v >> 5], 1u << (v & 31)) >> (v & 31)) & 1u)) flag |= 2u;
     }
-    const int flag = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (again ? 2u : 0u));
+    flag = __reduce_or_sync(0xffffffffu, flag);
     if (Tm::lane() == 0) flags[slot][Tm::warp()] = flag;
-    const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, inv_t);
-    if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
   }
   // the rest of the row
   Sums sum{neg_inf(), 0.f, 0.f};
   uint32_t now = chunk;
 #pragma unroll 1
   for (int base = share.begin; base < share.end || base == share.begin; base += cap) {
-    const int n = own_vectors<kThreads>(base, min(base + cap, share.end)), next = base + cap;
+    const int end = min(base + cap, share.end), n = own_vectors<kThreads>(base, end);
+    const int next = base + cap;
     if (chunks > 1 && next < share.end) {
       copy_chunk<T, kThreads>(2 * chunk + cap * 16 - now, row, next,
                               own_vectors<kThreads>(next, min(next + cap, share.end)));
@@ -1343,15 +1359,17 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     }
     if (kMask && base != share.begin) fetch_mask(base, 0, n);
     Tm::sync();                                   // the whole chunk is there
-    const int first = row.head + base * N, last = first + min(cap, share.end - base) * N;
+    const int first = row.head + base * N, last = first + (end - base) * N;
 #pragma unroll 1
     for (int k = Tm::tid(); k < K; k += kThreads) {
       const int v = idx[k];
       if (v >= first && v < last) sts_neg_inf<T>(now + (v - first) * (int)sizeof(T));
     }
     Tm::sync();
-    if (base == share.begin && Tm::warp() == Tm::kWarps - 1)   // wanted after the sums
-      join_list<kThreads>(lred[slot], factor[slot], list_warps, inv_t);
+    if (base == share.begin && Tm::warp() < list_warps) {
+      const ListSums ls = list_sums(p, zu, idx, K, Tm::tid(), 32 * list_warps, o.renormalize, inv_t);
+      if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
+    }
     uint32_t at = now + Tm::tid() * 16;
 #pragma unroll 1
     for (int i = 0; i < n; i += kBatch) {
@@ -1380,20 +1398,18 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     if (!in) sum = join(sum, single(edge, a.c), a.c);
   }
   int all = 0;
-  for (int w = 0; w < list_warps; ++w) all |= flags[slot][w];
+  for (int w = 0; w < load_warps; ++w) all |= flags[slot][w];
   if (all & 2) {                                  // an entry listed twice counts once
+    Tm::sync();
     for (int k = Tm::tid(); k < K; k += kThreads) p[k] = (double)o.log_probs[row.index * K + k];
     Tm::sync();
     merge_list<kThreads>(p, idx, K);
     if (Tm::warp() < list_warps) {
-      const ListSums ls = list_sums<kThreads>(p, zu, idx, K, o.renormalize, inv_t);
+      const ListSums ls = list_sums(p, zu, idx, K, Tm::tid(), 32 * list_warps, o.renormalize, inv_t);
       if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;
     }
-    Tm::sync();
-    if (Tm::warp() == 0) join_list<kThreads>(lred[slot], factor[slot], list_warps, inv_t);
-    Tm::sync();
   }
-  sum = team_sums<kThreads>(sum, a.c, red[slot]);   // orders lred, too (a barrier, or one warp)
+  sum = team_sums<kThreads>(sum, a.c, red[slot]);   // orders lred and p, too (a barrier, or one warp)
   if constexpr (kThreads == 32) __syncwarp();
   if (blocks > 1) {
     cluster_wait();
@@ -1407,17 +1423,24 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
 #pragma unroll 1
     for (int b = 1; b < blocks; ++b) sum = join(sum, Sums{cl[b][0], cl[b][1], 0.f}, a.c);
   }
-  const ListSums ls = K > 0 ? lred[slot][0] : ListSums{0.0, 0.0, 0.0, 0.0, neg_inf(), 0.f};
+  // P of the entries that this thread writes is warp (k / 32 mod list_warps)'s
+  float factor = 1.f;
+  ListSums ls{0.0, 0.0, 0.0, 0.f, neg_inf(), 0.f};
+  if (list_warps == 1) ls = lred[slot][0];
+  else if (list_warps > 1)
+    ls = join_list(lred[slot], list_warps, Tm::warp() % list_warps, inv_t, &factor);
   const bool rest = sum.m != neg_inf(), listed = ls.top_z != neg_inf();
-  bad = (all & 1) || sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
+  const bool bad = (all & 1) || sum.s != sum.s || ls.e != ls.e || ls.mass != ls.mass;
   const bool whole = o.renormalize || ls.mass > 1.0 || !rest;
-  const float inv = whole && ls.mass > 0.0 ? 1.f / (float)ls.mass : 1.f;
   const float p_r = whole ? 0.f : (float)(1.0 - ls.mass);
   const bool live = (rest || listed) && (ls.mass > 0.0 || !whole);
   // the two normalisers relative to the larger of the two maxima
   const float big = fmaxf(rest ? sum.m : neg_inf(), ls.top_z);
   const float norm_r = rest ? sum.s * ex2((sum.m - big) * a.c) : 0.f;
-  const float norm = norm_r + (listed ? (float)ls.e * ex2((ls.top_z - big) * a.c) : 0.f);
+  const float inv_norm =
+      __fdividef(1.f, norm_r + (listed ? ls.e * ex2((ls.top_z - big) * a.c) : 0.f));
+  const float scaled = weight * o.scale *
+                       (o.upstream ? o.upstream[row.index * o.upstream_stride] : 1.f);
   // by the last warp, when the others are done; a function call to a lane
   auto write_loss = [&]() {
     if (rank != 0 || Tm::warp() != Tm::kWarps - 1 || !o.row_loss) return;
@@ -1426,7 +1449,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     const double down_u = listed ? ((double)ls.top_z - (double)big) * inv_t : 0.0;
     const double rest_mass = whole ? 0.0 : 1.0 - ls.mass;
     double e = exp64(lane == 0 ? down_r : down_u);          // 0: the rest, 1: the list
-    e *= lane == 0 ? (rest ? (double)sum.s : 0.0) : (listed ? ls.e : 0.0);
+    e *= lane == 0 ? (rest ? (double)sum.s : 0.0) : (listed ? (double)ls.e : 0.0);
     const double norm64 = __shfl_sync(0xffffffffu, e, 0) + __shfl_sync(0xffffffffu, e, 1);
     const double l = log(lane == 0 ? norm64 : lane == 1 ? ls.mass : lane == 2 ? rest_mass
                                                                               : (double)sum.s);
@@ -1440,14 +1463,14 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     if (live && rest_mass > 0.0) loss += rest_mass * (log_p_r - (down_r + log_s - log_all));
     if (lane == 0)
       o.row_loss[row.index] =
-          bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)weight);
+          bad ? quiet_nan() : (float)(loss * (double)a.t * (double)a.t * (double)scaled);
   };
   if (!row.grad) {
     write_loss();
     return;
   }
-  const float scale = live ? weight * a.t : 0.f, ref = rest ? sum.m : 0.f;
-  const float coef = live && rest ? scale * (norm_r / norm - p_r) / sum.s : 0.f;
+  const float scale = live ? scaled * a.t : 0.f, ref = rest ? sum.m : 0.f;
+  const float coef = live && rest ? __fdividef(scale * (norm_r * inv_norm - p_r), sum.s) : 0.f;
   const float nan = bad || coef != coef ? quiet_nan() : 0.f;   // of a row without a distribution
   const float2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
   auto slope = [&](const uint4& r, int j) {
@@ -1493,13 +1516,15 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     row.grad[share.edge] =
         to_type<T>(edge == neg_inf() ? 0.f : nan + ex2((edge - ref) * a.c) * coef);
   if (K > 0) Tm::sync();                          // the listed entries are written again
+  if (Tm::warp() < load_warps) {
+    const double inv = whole && ls.mass > 0.0 ? (double)factor / ls.mass : (double)factor;
 #pragma unroll 1
-  for (int k = Tm::tid(); k < K; k += kThreads) {
-    const int v = idx[k];
-    if (v < share.first || v >= share.last) continue;
-    const float q = expf((zu[k] - big) * a.inv_t) / norm;
-    const float pk = (float)p[k] * factor[slot][Tm::warp()];
-    row.grad[v] = to_type<T>(nan + scale * (q - pk * inv));
+    for (int k = Tm::tid(); k < K; k += kThreads) {
+      const int v = idx[k];
+      if (v < share.first || v >= share.last) continue;
+      const float q = ex2((zu[k] - big) * a.c) * inv_norm;
+      row.grad[v] = to_type<T>(nan + scale * (q - (float)(p[k] * inv)));
+    }
   }
   write_loss();
 }
