@@ -41,6 +41,7 @@ template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
   static constexpr uint32_t kNegInf = 0xff800000u;
+  static constexpr uint32_t kFill = 0xf149f2cau;       // -1e30
   static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[4]) {
     f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y);
     f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
@@ -63,6 +64,7 @@ template <> struct Vec<float> {
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
   static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static constexpr uint32_t kFill = 0xf14af14au;       // -1e30
   static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[8]) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -99,6 +101,7 @@ template <> struct Vec<__nv_bfloat16> {
 template <> struct Vec<__half> {
   static constexpr int N = 8;
   static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static constexpr uint32_t kFill = 0xfbfffbffu;       // -65504, the lowest
   static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[8]) {
     const __half2* h = reinterpret_cast<const __half2*>(&r);
 #pragma unroll
@@ -134,9 +137,14 @@ template <> struct Vec<__half> {
   static __device__ __forceinline__ float max(const uint4& r) { return to_max(wide_max(r)); }
 };
 
-template <typename T>
-__device__ __forceinline__ uint4 neg_inf_vec() {
-  return make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
+template <uint32_t kBits> __device__ __forceinline__ uint4 vec_of() {
+  return make_uint4(kBits, kBits, kBits, kBits);
+}
+// a vector of a type's fill value, and that value
+template <typename T> __device__ __forceinline__ float fill_value() {
+  float f[Vec<T>::N];
+  Vec<T>::unpack(vec_of<Vec<T>::kFill>(), f);
+  return f[0];
 }
 
 // Shared memory by 32-bit address plus an offset known at compile time.
@@ -163,8 +171,8 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 constexpr int kBatch = 4;          // vectors that a thread takes at a time
 
 // A thread's next kBatch vectors of a row to a place in shared memory, both
-// kStride vectors apart; -inf for those behind its last.
-template <typename T, int kStride>
+// kStride vectors apart; kBits for those behind its last.
+template <int kStride, uint32_t kBits>
 __device__ __forceinline__ void copy_batch(uint32_t dst, const char* src, int left) {
   constexpr int S = kStride * 16;
   if (left >= kBatch) {
@@ -173,10 +181,10 @@ __device__ __forceinline__ void copy_batch(uint32_t dst, const char* src, int le
     copy16<2 * S, 2 * S>(dst, src);
     copy16<3 * S, 3 * S>(dst, src);
   } else {
-    if (left > 0) copy16<0, 0>(dst, src); else sts128<0>(dst, neg_inf_vec<T>());
-    if (left > 1) copy16<S, S>(dst, src); else sts128<S>(dst, neg_inf_vec<T>());
-    if (left > 2) copy16<2 * S, 2 * S>(dst, src); else sts128<2 * S>(dst, neg_inf_vec<T>());
-    sts128<3 * S>(dst, neg_inf_vec<T>());
+    if (left > 0) copy16<0, 0>(dst, src); else sts128<0>(dst, vec_of<kBits>());
+    if (left > 1) copy16<S, S>(dst, src); else sts128<S>(dst, vec_of<kBits>());
+    if (left > 2) copy16<2 * S, 2 * S>(dst, src); else sts128<2 * S>(dst, vec_of<kBits>());
+    sts128<3 * S>(dst, vec_of<kBits>());
   }
 }
 template <int kStride>
@@ -372,7 +380,7 @@ __device__ __forceinline__ void copy_chunk(uint32_t chunk, const Row<T>& row, in
   uint32_t dst = chunk + Team<kThreads>::tid() * 16;
 #pragma unroll 1
   for (; n > 0; n -= kBatch) {
-    copy_batch<T, kThreads>(dst, src, n);
+    copy_batch<kThreads, Vec<T>::kNegInf>(dst, src, n);
     dst += kBatch * kThreads * 16;
     src += kBatch * kThreads * 16;
   }
@@ -398,6 +406,8 @@ __device__ __forceinline__ Sums single(float z, float c) {
 // Adds vectors, whose maximum is `top`, to the running sums: per entry one
 // exponential and half an add, a product and a sum or two. With kClamp also a
 // clamp, for the entropy's 0 * -inf; without, t is NaN if there is a -inf.
+// Places without an entry hold the fill value, whose exponential is 0 unless
+// the maximum is as low.
 template <typename T, int kVecs, bool kEntropy, bool kClamp>
 __device__ __forceinline__ void accumulate(const uint4 (&r)[kVecs], float top, float c, Sums& a) {
   constexpr int N = Vec<T>::N;
@@ -442,6 +452,20 @@ __device__ __forceinline__ uint32_t logit_key(float z) {
 __device__ __forceinline__ float key_logit(uint32_t b) {
   return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
+// A thread's sums of a share whose entries are -inf in places, or all of them
+// as low as the fill value: clamped, and read from memory without any fill.
+template <typename T, int kThreads, bool kMask>
+__device__ __noinline__ Sums careful_sums(const Row<T>& row, const Share<T>& share, float c) {
+  Sums sum{neg_inf(), 0.f, 0.f};
+#pragma unroll 1
+  for (int j = share.begin + Team<kThreads>::tid(); j < share.end; j += kThreads) {
+    uint4 r[1] = {*reinterpret_cast<const uint4*>(row.vec(j))};
+    if (kMask) row.apply_mask(r[0], j);
+    accumulate<T, 1, true, true>(r, Vec<T>::max(r[0]), c, sum);
+  }
+  return sum;
+}
+
 // Joins the team's sums (every thread gets the result): the maximum first, so
 // that each thread rescales its own sums once.
 template <int kThreads>
@@ -491,7 +515,7 @@ struct Ring {
   // asks for the next batch into the half `at` of the ring
   __device__ __forceinline__ void ask(uint32_t at) {
     if (left > 0) {
-      copy_batch<T, kThreads>(at, src, left);
+      copy_batch<kThreads, Vec<T>::kFill>(at, src, left);
       src += kBatch * kThreads * 16;
       left -= kBatch;
     }
@@ -509,7 +533,7 @@ __device__ __forceinline__ int key_index(unsigned long long key) {
 
 template <int kThreads> struct TopShared {
   static constexpr int kMaxCand = 512;
-  unsigned long long cand[kMaxCand];
+  alignas(16) unsigned long long cand[kMaxCand];
   uint32_t bound[Team<kThreads>::kWarps];
   uint4 hold[Team<kThreads>::kWarps][32];
   int hold_at[Team<kThreads>::kWarps][32];
@@ -702,6 +726,7 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
       }
     }
   }
+  if (lo <= logit_key(fill_value<T>())) lo = 0;   // places without an entry may be among them
   const float least = lo ? key_logit(lo) : -3.4028234664e38f;   // the lowest logit there is
   // the groups that reach it, warp by warp: their vectors, one to a lane
   uint8_t* list = sh.list[Tm::warp()];
@@ -724,6 +749,7 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
   const int lg = per > 16 ? 5 : per > 1 ? 32 - __clz(per - 1) : 0;
   const int g_lane = Tm::lane() >> lg, g_step = 32 >> lg, i_lane = Tm::lane() & ((1 << lg) - 1);
   const uint32_t before = (1u << Tm::lane()) - 1;
+  int found = 0;                                       // a team of one warp needs no shared count
 #pragma unroll 1
   for (int g0 = 0; g0 < groups; g0 += kBatch * g_step) {
 #pragma unroll 1
@@ -761,15 +787,24 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
           if (t < entries) z = to_float(reinterpret_cast<const T*>(hold)[t]);
           const bool top_z = z >= least;
           const uint32_t hits = __ballot_sync(kAll, top_z);
-          int at = 0;
-          if (Tm::lane() == 0) at = atomicAdd(&sh.count, __popc(hits));
-          at = __shfl_sync(kAll, at, 0) + __popc(hits & before);
+          int at = found;
+          if constexpr (kThreads == 32) {
+            found += __popc(hits);
+          } else {
+            if (Tm::lane() == 0) at = atomicAdd(&sh.count, __popc(hits));
+            at = __shfl_sync(kAll, at, 0);
+          }
+          at += __popc(hits & before);
           if (top_z && at < TopShared<kThreads>::kMaxCand)
             sh.cand[at] = order_key(logit_key(z), hold_at[t / N] + (t & (N - 1)));
         }
         __syncwarp();
       }
     }
+  }
+  if constexpr (kThreads == 32) {
+    if (Tm::lane() == 0) sh.count = found;
+    __syncwarp();
   }
   if (share.edge >= 0 && edge >= least) {
     const int at = atomicAdd(&sh.count, 1);
@@ -786,8 +821,13 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
 __device__ __forceinline__ int rank_of(unsigned long long key, const unsigned long long* keys,
                                        int n) {
   int r = 0;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) r += keys[i] > key;
+#pragma unroll 2
+  for (int i = 0; i + 1 < n; i += 2) {
+    const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + i);
+    r += two.x > key;
+    r += two.y > key;
+  }
+  if (n & 1) r += keys[n - 1] > key;
   return r;
 }
 
@@ -825,9 +865,9 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
   constexpr uint32_t kHalf = kBatch * kThreads * 16;
   ring.ask(at);
   ring.ask(at + kHalf);
+  // single entries and the first given ones are fetched while the row is on its way
   float edge = neg_inf();
   if (share.edge >= 0) edge = row.at(share.edge);
-  // the first given entries are fetched while the row is on its way
   long long given[2];
   float given_z[2];
 #pragma unroll
@@ -836,14 +876,18 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
     given[q] = -1;
     given_z[q] = 0.f;
     if (rank == 0 && k < o.n_targets) given[q] = o.targets[row.index * o.n_targets + k];
-    if (given[q] >= 0 && given[q] < row.size) given_z[q] = row.at((int)given[q]);
   }
-  Sums sum = single(edge, a.c);
+  auto fetch_given = [&]() {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (given[q] >= 0 && given[q] < row.size) given_z[q] = row.at((int)given[q]);
+  };
+  if (ring.n == 0) fetch_given();
+  Sums sum{neg_inf(), 0.f, 0.f};
   typename Vec<T>::Max tops[kBatch];
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) tops[u] = Vec<T>::lowest();
   const bool keep = kMask && share.end - share.begin <= kSlots * kThreads;
-  bool clamp = kMask;                             // this thread has met a -inf
   typename Row<T>::MaskBytes ahead[kBatch];       // of the next batch
   auto fetch_mask = [&](int i) {
 #pragma unroll
@@ -877,16 +921,13 @@ log_probs_kernel(const __grid_constant__ Rows a, const ScoreArgs o, unsigned row
     asm volatile("" ::"f"(all) : "memory");
     ring.ask(at);
     at = at == ring.buf ? at + kHalf : ring.buf;
-    if (!clamp) {
-      const Sums before = sum;
-      accumulate<T, kBatch, true, false>(r, all, a.c, sum);
-      if (sum.t != sum.t) {
-        clamp = true;
-        sum = before;
-      }
-    } 
-    if (clamp) accumulate<T, kBatch, true, true>(r, all, a.c, sum);
+    accumulate<T, kBatch, true, kMask>(r, all, a.c, sum);
+    if (i == 0) fetch_given();
   }
+  // entries of -inf, or a maximum as low as the fill value
+  if (sum.t != sum.t || !((sum.m - fill_value<T>()) * a.c > 64.f))
+    sum = careful_sums<T, kThreads, kMask>(row, share, a.c);
+  if (share.edge >= 0) sum = join(sum, single(edge, a.c), a.c);
   cp_async_wait<0>();
   sum = team_sums<kThreads>(sum, a.c, sh.red);
   int n = 0;
