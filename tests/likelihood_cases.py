@@ -388,3 +388,89 @@ def case_no_second_derivative(dev):
     g, = torch.autograd.grad(out.entropy.sum(), z, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+# ------------------------------------------------------------ rows that take the rarer ways
+def case_hard_rows(dev, dtype, v, k):
+    """Rows whose largest entries lie in one place, in order, or are few; rows with -inf."""
+    g = torch.Generator().manual_seed(v + k)
+    noise = torch.randn(9, v, generator=g)
+    pos = torch.arange(v).float()
+    z = torch.stack([
+        pos / v * 8 + noise[0] * 1e-3,                                # ascending
+        -pos / v * 8 + noise[1] * 1e-3,                               # descending
+        8 * torch.exp(-((pos - v // 3) / 12) ** 2) + noise[2] * 0.1,  # a summit
+        8 * torch.exp(-((pos - v // 2) / (v / 5)) ** 2) + noise[3] * 0.1,   # a broad one
+        torch.where(pos % max(2, v // 7) == 3, noise[4], -INF),       # few entries at all
+        torch.where(torch.rand(v, generator=g) < 0.5, noise[5], -INF),
+        torch.where(pos == v - 1, 2.0, -INF),                         # one entry, at the end
+        torch.full((v,), -INF),
+        torch.full((v,), float(torch.finfo(dtype).min)),
+    ]).to(dtype)
+    t = C.make_targets((9, v), None, 3, g)
+    t[:, 0] = v - 1
+    z, t = z.to(dev).requires_grad_(), t.to(dev)
+    out = cb.profile_log_probs(z, t, top_k=k)
+    gs = dict(lp=torch.randn(t.shape, generator=g), h=torch.randn(9, generator=g),
+              norm=torch.randn(9, generator=g), top=torch.randn(9, k, generator=g))
+    gs = {n: x.to(dev) for n, x in gs.items()}
+    grad, = torch.autograd.grad(out[:4], z, tuple(gs.values()))
+    C.check_scores(z, out, t, k, None, None, 1.0, gs, grad)
+    idx, lp = out.top_indices, out.top_log_probs.detach().clamp(min=-60.0) - 0.05
+    for renorm in (False, True):
+        loss, grad = cb.distillation_loss_and_grad(z, idx, lp, renormalize=renorm,
+                                                   reduction="none")
+        C.check_distill(z, idx, lp, renorm, None, None, 1.0, None, "none", loss, grad)
+
+
+def case_repeats(dev, v, k, rows):
+    """Lists with entries twice and more, next to lists where they only look alike (32768 apart),
+    empty places and dropped entries among them."""
+    z, g = C.logits((rows, v), F32, v + k)
+    z[:, ::11] = -INF
+    idx = torch.randint(0, v, (rows, k), generator=g)
+    idx[:, 1::5] = idx[:, 0:1]
+    idx[:, 2::7] = torch.where(idx[:, 3:4] >= 32768, idx[:, 3:4] - 32768,
+                               (idx[:, 3:4] + 32768) % v)
+    idx[:, 4::9] = -1
+    lp = torch.log_softmax(torch.randn(rows, k, generator=g), -1) - 0.2
+    lp[:, 5::13] = -INF
+    z, idx, lp = z.to(dev), idx.to(dev), lp.to(dev)
+    w = torch.ones(rows)
+    if rows > 2:
+        w[1] = 0.0
+    w = w.to(dev)
+    for renorm in (False, True):
+        how = dict(renormalize=renorm, weight=w, reduction="none")
+        loss, grad = cb.distillation_loss_and_grad(z, idx, lp, **how)
+        C.check_distill(z, idx, lp, renorm, None, None, 1.0, w, "none", loss, grad)
+        C.check_distill(z, idx, lp, renorm, None, None, 1.0, w, "none",
+                        cb.distillation_loss(z, idx, lp, **how), None)
+
+
+def case_many_targets(dev, v):
+    """As many given entries as a call takes, most of them more than once."""
+    z, g = C.logits((2, v), BF16, 3)
+    t = torch.randint(0, min(v, 300), (2, 1024), generator=g)
+    t[:, ::17] = -1
+    z, t = z.to(dev).requires_grad_(), t.to(dev)
+    out = cb.profile_log_probs(z, t)
+    gs = dict(lp=torch.randn(t.shape, generator=g), h=torch.zeros(2), norm=torch.zeros(2),
+              top=torch.zeros(2, 0))
+    grad, = torch.autograd.grad(out.log_probs, z, gs["lp"].to(dev))
+    C.check_scores(z, out, t, 0, None, None, 1.0, gs, grad)
+
+
+def case_temperatures(dev, dtype, T):
+    z, g = C.logits((3, 700), dtype, 41)
+    z[1] = -torch.finfo(dtype).max
+    z[1, 5:9] = -torch.finfo(dtype).max * 0.75
+    t = C.make_targets((3, 700), None, 2, g).to(dev)
+    z = z.to(dev)
+    out = cb.profile_log_probs(z, t, top_k=9, temperature=T)
+    C.check_scores(z, out, t, 9, None, None, T)
+    idx = out.top_indices
+    lp = out.top_log_probs.clamp(min=-80.0)
+    loss, grad = cb.distillation_loss_and_grad(z[::2], idx[::2], lp[::2] - 0.1, temperature=T,
+                                               reduction="none")
+    C.check_distill(z[::2], idx[::2], lp[::2] - 0.1, False, None, None, T, None, "none", loss, grad)

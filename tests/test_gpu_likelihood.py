@@ -289,3 +289,50 @@ def test_long_strides():
     loss, grad = cb.distillation_loss_and_grad(view, out.top_indices, out.top_log_probs - 0.1)
     C.check_distill(view, out.top_indices, out.top_log_probs - 0.1, False, None, None, 1.0, None,
                     "mean", loss, grad)
+
+
+# a warp, a block and a cluster to a row; below and above what a ring or a chunk holds
+@pytest.mark.parametrize("dtype", [K.F32, K.BF16, K.F16])
+@pytest.mark.parametrize("v,k", [(50, 7), (403, 50), (900, 40), (2000, 64), (2100, 128),
+                                 (9001, 20), (70001, 64), (300001, 128)])
+def test_hard_rows(dtype, v, k):
+    K.case_hard_rows(DEV, dtype, v, k)
+
+
+@pytest.mark.parametrize("v,k,rows", [(60, 20, 3), (1000, 128, 3), (3001, 129, 3),
+                                      (12000, 400, 3), (70000, 90, 3), (70000, 1024, 2),
+                                      (300000, 700, 2), (40000, 300, 300)])
+def test_repeats(v, k, rows):
+    K.case_repeats(DEV, v, k, rows)
+
+
+@pytest.mark.parametrize("v", [2000, 40000])
+def test_many_targets(v):
+    K.case_many_targets(DEV, v)
+
+
+@pytest.mark.parametrize("T", [1 / 1024, 1024.0])
+@pytest.mark.parametrize("dtype", [K.F32, K.BF16, K.F16])
+def test_temperatures(dtype, T):
+    K.case_temperatures(DEV, dtype, T)
+
+
+@pytest.mark.parametrize("dtype", [K.F32, K.BF16])
+def test_windows_and_masks_off_their_boundaries(dtype):
+    """Logits, mask and gradient whose rows start at every offset from a 16-byte boundary."""
+    g = torch.Generator().manual_seed(7)
+    for off in range(8):
+        for width in (45, 1500, 6007):
+            full = torch.randn(3, width + 16 + off % 3, generator=g).to(dtype).to(DEV)
+            z = full[:, off:off + width].requires_grad_()
+            m = torch.rand(3, width + 9, generator=g).to(DEV)[:, (5 * off) % 8:][:, :width] < 0.7
+            t = C.make_targets(z.shape, None, 3, g).to(DEV)
+            out = cb.profile_log_probs(z, t, top_k=6, mask=m)
+            gs = dict(lp=torch.randn(t.shape, generator=g), h=torch.randn(3, generator=g),
+                      norm=torch.randn(3, generator=g), top=torch.randn(3, 6, generator=g))
+            gs = {n: v.to(DEV) for n, v in gs.items()}
+            grad, = torch.autograd.grad(out[:4], z, tuple(gs.values()))
+            C.check_scores(z, out, t, 6, m, None, 1.0, gs, grad)
+            lp = out.top_log_probs.detach() - 0.1
+            loss, grad = cb.distillation_loss_and_grad(z, out.top_indices, lp, mask=m)
+            C.check_distill(z, out.top_indices, lp, False, m, None, 1.0, None, "mean", loss, grad)

@@ -104,3 +104,23 @@ def test_abi_rejects_before_any_launch():
     assert distill(rows(), k=-1) == 1 and distill(rows(), k=1025) == 1
     assert distill(rows(), stride=2) == 1
     assert distill(rows(), row_loss=None, loss=bogus) == 1
+
+
+@pytest.mark.parametrize("v,k", [(50, 7), (900, 40)])
+def test_hard_rows(v, k):
+    K.case_hard_rows(DEV, K.F32, v, k)
+
+
+@pytest.mark.parametrize("v,k", [(60, 20), (70000, 90)])
+def test_repeats(v, k):
+    K.case_repeats(DEV, v, k, 3)
+
+
+def test_many_targets():
+    K.case_many_targets(DEV, 2000)
+
+
+@pytest.mark.parametrize("T", [1 / 1024, 1024.0])
+@pytest.mark.parametrize("dtype", [K.F32, K.F16])
+def test_temperatures(dtype, T):
+    K.case_temperatures(DEV, dtype, T)
