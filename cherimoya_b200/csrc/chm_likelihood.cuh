@@ -694,7 +694,7 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
     // 32 maxima reach the smallest of the lanes' largest
     if (want <= 32) lo = __reduce_min_sync(kAll, most);
     uint32_t hi = __reduce_max_sync(kAll, most) + 1;
-    for (int n = 128; hi - lo > 1 && n > want + want / 4;) {
+    for (int n = 128; hi - lo > 1 && n > want + want / 16;) {
       const uint32_t mid = lo + (hi - lo) / 2;
       const int r = __reduce_add_sync(kAll, reach(mid));
       if (r >= want) {
@@ -750,57 +750,57 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
   const int g_lane = Tm::lane() >> lg, g_step = 32 >> lg, i_lane = Tm::lane() & ((1 << lg) - 1);
   const uint32_t before = (1u << Tm::lane()) - 1;
   int found = 0;                                       // a team of one warp needs no shared count
+  const int rounds = (groups + g_step - 1) / g_step * ((per + 31) / 32);
+  // the vector that this lane has in a round: its place in the share, or -1
+  auto fetch = [&](int round, uint4& r) {
+    const int parts = (per + 31) / 32, i_at = (parts == 1 ? 0 : round % parts * 32) + i_lane;
+    const int g = (parts == 1 ? round : round / parts) * g_step + g_lane;
+    if (round >= rounds || g >= groups || i_at >= per) return -1;
+    const int who = list[g], i = i_at * kBatch + (who & (kBatch - 1));
+    const int j = share.begin + i * kThreads + Tm::warp() * 32 + who / kBatch;
+    if (j >= share.end) return -1;
+    if (here) r = lds128<0>(slots + (i * kThreads + who / kBatch) * 16);
+    else r = __ldg(reinterpret_cast<const uint4*>(row.vec(j)));
+    return j;
+  };
+  uint4 r0, r1, r2;                                    // of this round and the next two
+  int j0 = fetch(0, r0), j1 = fetch(1, r1);
 #pragma unroll 1
-  for (int g0 = 0; g0 < groups; g0 += kBatch * g_step) {
-#pragma unroll 1
-    for (int i0 = 0; i0 < per; i0 += 32) {
-      uint4 r[kBatch];
-      int j[kBatch];
-#pragma unroll
-      for (int x = 0; x < kBatch; ++x) {
-        const int g = g0 + x * g_step + g_lane;
-        const int who = list[min(g, groups - 1)];
-        const int i = (i0 + i_lane) * kBatch + (who & (kBatch - 1));
-        j[x] = share.begin + i * kThreads + Tm::warp() * 32 + who / kBatch;
-        if (g >= groups || i0 + i_lane >= per || j[x] >= share.end) j[x] = -1;
-        else if (here) r[x] = lds128<0>(slots + (i * kThreads + who / kBatch) * 16);
-        else r[x] = __ldg(reinterpret_cast<const uint4*>(row.vec(j[x])));
-      }
-#pragma unroll
-      for (int x = 0; x < kBatch; ++x) {
-        if (g0 + x * g_step >= groups) break;
-        if (kMask && !here && j[x] >= 0) row.apply_mask(r[x], j[x]);
-        const bool in = j[x] >= 0 && Vec<T>::max(r[x]) >= least;
-        const uint32_t vote = __ballot_sync(kAll, in);
-        if (!vote) continue;
-        // the vectors that reach the bound side by side, then one entry to a lane
-        if (in) {
-          hold[__popc(vote & before)] = r[x];
-          hold_at[__popc(vote & before)] = row.head + j[x] * N;
-        }
-        __syncwarp();
-        const int entries = __popc(vote) * N;
-#pragma unroll 1
-        for (int t0 = 0; t0 < entries; t0 += 32) {
-          const int t = t0 + Tm::lane();
-          float z = neg_inf();
-          if (t < entries) z = to_float(reinterpret_cast<const T*>(hold)[t]);
-          const bool top_z = z >= least;
-          const uint32_t hits = __ballot_sync(kAll, top_z);
-          int at = found;
-          if constexpr (kThreads == 32) {
-            found += __popc(hits);
-          } else {
-            if (Tm::lane() == 0) at = atomicAdd(&sh.count, __popc(hits));
-            at = __shfl_sync(kAll, at, 0);
-          }
-          at += __popc(hits & before);
-          if (top_z && at < TopShared<kThreads>::kMaxCand)
-            sh.cand[at] = order_key(logit_key(z), hold_at[t / N] + (t & (N - 1)));
-        }
-        __syncwarp();
-      }
+  for (int round = 0; round < rounds; ++round) {
+    const int j2 = fetch(round + 2, r2);
+    if (kMask && !here && j0 >= 0) row.apply_mask(r0, j0);
+    const bool in = j0 >= 0 && Vec<T>::max(r0) >= least;
+    const uint32_t vote = __ballot_sync(kAll, in);
+    // the vectors that reach the bound side by side, then one entry to a lane
+    if (in) {
+      hold[__popc(vote & before)] = r0;
+      hold_at[__popc(vote & before)] = row.head + j0 * N;
     }
+    __syncwarp();
+    const int entries = __popc(vote) * N;
+#pragma unroll 1
+    for (int t0 = 0; t0 < entries; t0 += 32) {
+      const int t = t0 + Tm::lane();
+      float z = neg_inf();
+      if (t < entries) z = to_float(reinterpret_cast<const T*>(hold)[t]);
+      const bool top_z = z >= least;
+      const uint32_t hits = __ballot_sync(kAll, top_z);
+      int at = found;
+      if constexpr (kThreads == 32) {
+        found += __popc(hits);
+      } else {
+        if (Tm::lane() == 0) at = atomicAdd(&sh.count, __popc(hits));
+        at = __shfl_sync(kAll, at, 0);
+      }
+      at += __popc(hits & before);
+      if (top_z && at < TopShared<kThreads>::kMaxCand)
+        sh.cand[at] = order_key(logit_key(z), hold_at[t / N] + (t & (N - 1)));
+    }
+    __syncwarp();
+    r0 = r1;
+    j0 = j1;
+    r1 = r2;
+    j1 = j2;
   }
   if constexpr (kThreads == 32) {
     if (Tm::lane() == 0) sh.count = found;
