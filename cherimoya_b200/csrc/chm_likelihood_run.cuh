@@ -21,9 +21,16 @@ struct Cut {
 
 int largest(const Rows& a) { return *std::max_element(a.size, a.size + a.ng); }
 
-// A warp takes a short row, a block of 128, 256 or 512 threads a longer one;
-// rows of more than kChunkBytes are shared by the blocks of a cluster, so that
-// each holds its share, and few long rows are cut further, to reach more SMs.
+// Distillation with a gradient keeps a block's share of a row in shared memory
+// from the first look to the last, so the row's size sets how many blocks an
+// SM holds. A warp takes a short row and a block of 128 one of up to 44 KB, of
+// which five fit: 8,192 x 20,000 bf16 entries take 147 us with it and 185 with
+// 256 threads, 8,192 x 9,000 take 108 and 150; 8,192 x 32,768, of which
+// three fit, take 220 with 256 threads, 267 with 128 and 326 with 512, which
+// only rows above that get. Rows of more than kChunkBytes are shared by the
+// blocks of a cluster, so that each holds its share; few long rows are cut
+// further, to reach more SMs. Many rows are not (8,192 x 32,768 in clusters of
+// two: 387 us).
 constexpr int kChunkBytes = 96 << 10;
 Cut cut_rows(int nvec, long long rows, bool warp) {
   Cut c{};
@@ -31,15 +38,19 @@ Cut cut_rows(int nvec, long long rows, bool warp) {
   while (c.log_blocks < 3 && rows << c.log_blocks < 2 * 148 && nvec > 512 << c.log_blocks)
     ++c.log_blocks;
   const int share = (nvec + (1 << c.log_blocks) - 1) >> c.log_blocks;
-  c.threads = warp && share <= 256 ? 32 : share <= 1024 ? 128 : share <= 4096 ? 256 : 512;
+  c.threads = warp && share <= 256 ? 32 : share <= 2816 ? 128 : share <= 4096 ? 256 : 512;
   if (c.log_blocks && c.threads < 256) c.threads = 256;
   const int most = std::min(std::max(share, 1), kChunkBytes / 16);
   c.cap = (most + kBatch * c.threads - 1) / (kBatch * c.threads) * (kBatch * c.threads);
   return c;
 }
 
-// For the kernels that read a row once, a warp up to 16 vectors a lane, else a
-// block of 128, of which several share a row where there are few.
+// The log probabilities read a row once, through a ring of fixed size. A warp
+// takes up to 16 vectors a lane: 2,048 examples of five groups of 1,000 and 2,000
+// masked fp32 entries take 50 us, 56 with teams of 64 and 79 with 128. Longer rows get
+// a block of 128 (4,096 x 50,001 bf16: 88 us, 109 with 256), more than 64 top
+// entries too, since a lane keeps at most two; few long rows are shared by the
+// blocks of a cluster.
 Cut cut_stream(int nvec, long long rows, int top_k) {
   Cut c{};
   c.threads = nvec <= 512 && top_k <= 64 ? 32 : 128;
@@ -146,10 +157,13 @@ int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t
   const int nvec = largest(a) / Vec<T>::N;
   Cut c = cut_rows(nvec, n, o.n_listed <= 128);
   int chunks = 1;
-  if (!a.grad && nvec > 4096) {
-    // nothing is looked at twice: two chunks of 32 KB in turn, by one block where rows abound
-    c = {256, 0, 2048};
-    while (c.log_blocks < 3 && n << c.log_blocks < 3 * 148 && nvec >> c.log_blocks > 4096)
+  if (!a.grad && nvec > 1024) {
+    // Without a gradient nothing is looked at twice, so a block of 128 takes
+    // chunks of 16 KB, the next on its way while it sums one: 4,096 x 25,000 fp32
+    // entries take 82 us (32 KB and 256 threads: 104), 2,048 x 100,003 bf16 103
+    // (118), 8,192 x 12,000 84 (held whole: 120). Below 16 KB a row is one chunk.
+    c = {128, 0, 1024};
+    while (c.log_blocks < 3 && n << c.log_blocks < 3 * 148 && nvec >> c.log_blocks > 2048)
       ++c.log_blocks;
     chunks = 2;
   }
