@@ -325,6 +325,44 @@ template <int kThreads> struct Team {
   }
 };
 
+// A list of entries in the order of the row, each with its place in the list:
+// repeats are neighbours, the first of them first. Bitonic, over n keys, a
+// power of two; keys behind the list are kNoKey.
+constexpr uint32_t kNoKey = 0xffffffffu;
+constexpr int kPlaceBits = 11;                         // of a list of up to 2,048
+static_assert(kMaxList + kMaxTop <= 1 << kPlaceBits, "entries are below 2^20");
+__host__ __device__ constexpr int sort_size(int n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+__device__ __forceinline__ uint32_t place_key(int v, int place) {
+  return v < 0 ? kNoKey : (uint32_t)v << kPlaceBits | (uint32_t)place;
+}
+__device__ __forceinline__ int key_entry(uint32_t key) { return (int)(key >> kPlaceBits); }
+__device__ __forceinline__ int key_place(uint32_t key) {
+  return (int)(key & ((1u << kPlaceBits) - 1));
+}
+template <int kThreads> __device__ __noinline__ void sort_places(uint32_t* key, int n) {
+  using Tm = Team<kThreads>;
+#pragma unroll 1
+  for (int run = 2; run <= n; run *= 2)
+#pragma unroll 1
+    for (int half = run / 2; half > 0; half /= 2) {
+      Tm::sync();
+#pragma unroll 1
+      for (int t = Tm::tid(); t < n / 2; t += kThreads) {
+        const int i = (t & ~(half - 1)) * 2 + (t & (half - 1));
+        const uint32_t x = key[i], y = key[i + half];
+        if ((x > y) == ((i & run) == 0)) {
+          key[i] = y;
+          key[i + half] = x;
+        }
+      }
+    }
+  Tm::sync();
+}
+
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 }
@@ -1040,22 +1078,25 @@ __device__ __noinline__ void fill_bad(const Row<T>& row, const Share<T>& share) 
 // with a = g_norm - the sum of all incoming gradients of single entries. With
 // the forward's m and s that is e (A + B x) for the first term: one
 // exponential and two products per entry, and no reduction over the row.
-// Dynamic shared memory: per team the spots' indices and gradients.
+// Single entries with a gradient of their own are written again at the end, each
+// by one thread that adds up its gradients in the order of the list.
+// Dynamic shared memory: per team the spots' sorted keys and their gradients.
 template <typename T, int kThreads, bool kMask>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock)
 log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, unsigned rows,
                       int log_blocks) {
   using Tm = Team<kThreads>;
   constexpr int N = Vec<T>::N, kVecs = 4;
-  extern __shared__ int spots[];
+  extern __shared__ uint32_t spots[];
   __shared__ float red[Tm::kPerBlock][Tm::kWarps];
   const unsigned r0 = (blockIdx.x >> log_blocks) * Tm::kPerBlock + Tm::slot();
   if (kThreads == 32 && r0 >= rows) return;
   const Row<T> row(a, r0);
   const Share<T> share(row, blockIdx.x & ((1 << log_blocks) - 1), log_blocks, Tm::tid());
   const int nt = o.g_log_probs ? o.n_targets : 0, n = nt + (o.g_top ? o.top_k : 0);
-  int* idx = spots + Tm::slot() * 2 * n;
-  float* g = reinterpret_cast<float*>(idx + n);
+  const int keys = sort_size(n);
+  uint32_t* key = spots + Tm::slot() * (keys + n);
+  float* g = reinterpret_cast<float*>(key + keys);
   const float m = o.stats[2 * row.index], s = o.stats[2 * row.index + 1];
   float sum = 0.f;
 #pragma unroll 1
@@ -1068,10 +1109,11 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
     const bool past = i >= row.size;
     if (past) gk = quiet_nan();
     else if (i < 0 || row.at((int)i) == neg_inf()) gk = 0.f;
-    idx[k] = i < 0 || past ? -1 : (int)i;
+    key[k] = place_key(past ? -1 : (int)i, k);
     g[k] = gk;
     sum += gk;
   }
+  for (int k = n + Tm::tid(); k < keys; k += kThreads) key[k] = kNoKey;
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
   if (Tm::lane() == 0) red[Tm::slot()][Tm::warp()] = sum;
@@ -1128,29 +1170,28 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
   };
   if (share.edge >= 0) put(share.edge, 0.f);
   if (n == 0) return;
-  Tm::sync();                                     // the spots' entries are written again
+  sort_places<kThreads>(key, keys);               // and the entries are written before they are again
 #pragma unroll 1
   for (int k = Tm::tid(); k < n; k += kThreads) {
-    const int v = idx[k];
-    if (v < share.first || v >= share.last) continue;
-    bool first = true;
-    for (int q = 0; q < k; ++q) first &= idx[q] != v;
-    if (!first) continue;
+    const int v = key_entry(key[k]);
+    if (v < share.first || v >= share.last || (k > 0 && key_entry(key[k - 1]) == v)) continue;
     float at = 0.f;
-    for (int q = k; q < n; ++q) at += idx[q] == v ? g[q] : 0.f;
+    for (int q = k; q < n && key_entry(key[q]) == v; ++q) at += g[key_place(key[q])];
     put(v, at);
   }
 }
 
 // ------------------------------------------------------------ distillation
 // Shared memory of one team, in this order (dynamic): one or two chunks; p,
-// logits, indices of the list; a bit per entry of the row (modulo kSeenBits).
+// logits, indices of the list; a bit per entry of the row (modulo kSeenBits),
+// or the list's keys when they are sorted.
 constexpr int kSeenBits = 1 << 15;
 __host__ __device__ constexpr int seen_words(int size) {
   return ((size < kSeenBits ? size : kSeenBits) + 31) / 32;
 }
 __host__ __device__ constexpr int distill_bytes(int listed, int cap, int chunks, int largest) {
-  return chunks * cap * 16 + 16 * listed + (seen_words(largest) * 4 + 15) / 16 * 16;
+  const int words = seen_words(largest), keys = sort_size(listed);
+  return chunks * cap * 16 + 16 * listed + ((words > keys ? words : keys) * 4 + 15) / 16 * 16;
 }
 
 template <typename T> __device__ __forceinline__ void sts_neg_inf(uint32_t a) {
@@ -1255,37 +1296,29 @@ static __device__ __noinline__ ListSums join_list(const ListSums* part, int warp
 
 // A list in which an entry may be twice: the first one takes the others' mass
 // (p: log P before and after), the others leave the list. Marks can coincide
-// without a repeat, so most calls find none.
+// without a repeat, so there may be none.
 template <int kThreads>
-__device__ __noinline__ void merge_list(double* p, int* idx, int K) {
+__device__ __noinline__ void merge_list(double* p, int* idx, uint32_t* key, int K) {
   using Tm = Team<kThreads>;
-  uint32_t gone = 0;                              // of this thread's entries, in order
+  const int n = sort_size(K);
+  for (int k = Tm::tid(); k < n; k += kThreads) key[k] = k < K ? place_key(idx[k], k) : kNoKey;
+  sort_places<kThreads>(key, n);
 #pragma unroll 1
-  for (int k = Tm::tid(), i = 0; k < K; k += kThreads, ++i) {
-    const int v = idx[k];
-    if (v < 0) continue;
-    bool first = true;
-    for (int q = 0; q < k && first; ++q) first = idx[q] != v;
-    if (!first) {
-      gone |= 1u << i;
+  for (int k = Tm::tid(); k + 1 < K; k += kThreads) {
+    const int v = key_entry(key[k]);
+    if (key[k] == kNoKey || key_entry(key[k + 1]) != v || (k > 0 && key_entry(key[k - 1]) == v))
       continue;
+    const int first = key_place(key[k]);
+    double top = p[first], mass = 0.0;
+    for (int q = k + 1; q < K && key_entry(key[q]) == v; ++q)
+      top = fmax(top, p[key_place(key[q])]);
+    for (int q = k; q < K && key_entry(key[q]) == v; ++q) {
+      const int at = key_place(key[q]);
+      mass += exp64(p[at] - top);
+      if (q > k) idx[at] = -1;
     }
-    double top = p[k];
-    for (int q = k + 1; q < K; ++q)
-      if (idx[q] == v) top = fmax(top, p[q]);
-    double mass = exp64(p[k] - top);
-    bool alone = true;
-    for (int q = k + 1; q < K; ++q)
-      if (idx[q] == v) {
-        mass += exp64(p[q] - top);
-        alone = false;
-      }
-    if (!alone && top > (double)neg_inf()) p[k] = top + log(mass);
+    if (top > (double)neg_inf()) p[first] = top + log(mass);
   }
-  Tm::sync();
-#pragma unroll 1
-  for (int k = Tm::tid(), i = 0; k < K; k += kThreads, ++i)
-    if ((gone >> i) & 1u) idx[k] = -1;
   Tm::sync();
 }
 
@@ -1299,10 +1332,11 @@ __device__ __noinline__ void merge_list(double* p, int* idx, int K) {
 // so the gradient is one more exponential per entry in shared memory. Without
 // a gradient the chunks are small and there are two, one on its way.
 // The first warps add up the list while the others begin with the row.
-// At least three blocks of 256 to an SM, which 64 KB of shared memory allow.
+// At least three blocks of 256 to an SM, which 64 KB of shared memory allow, and
+// seven of 128.
 template <typename T, int kThreads, bool kMask>
 __global__ void
-__launch_bounds__(Team<kThreads>::kBlock, kThreads == 512 ? 1 : kThreads == 256 ? 3 : 5)
+__launch_bounds__(Team<kThreads>::kBlock, kThreads == 256 ? 3 : kThreads == 128 ? 7 : 5)
 distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned rows, int log_blocks,
                int cap, int chunks, int team_bytes) {
   using Tm = Team<kThreads>;
@@ -1432,11 +1466,18 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     if (chunks > 1) now = 2 * chunk + cap * 16 - now;
   }
   float edge = neg_inf();
-  if (share.edge >= 0) {
-    edge = row.at(share.edge);
-    bool in = false;
-    for (int k = 0; k < K; ++k) in |= idx[k] == share.edge;
-    if (!in) sum = join(sum, single(edge, a.c), a.c);
+  if (Tm::warp() == 0 && row.size != row.nin * N) {
+    // which single entries are listed: a bit per thread that may have one
+    if (share.edge >= 0) edge = row.at(share.edge);
+    const int tail = row.head + row.nin * N;
+    uint32_t in = 0;
+    for (int k = Tm::lane(); k < K; k += 32) {
+      const int v = idx[k];
+      if (v >= 0 && v < row.head) in |= 1u << v;
+      else if (v >= tail) in |= 1u << (N + v - tail);
+    }
+    in = __reduce_or_sync(0xffffffffu, in);
+    if (share.edge >= 0 && !((in >> Tm::tid()) & 1u)) sum = join(sum, single(edge, a.c), a.c);
   }
   int all = 0;
   for (int w = 0; w < load_warps; ++w) all |= flags[slot][w];
@@ -1444,7 +1485,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     Tm::sync();
     for (int k = Tm::tid(); k < K; k += kThreads) p[k] = (double)o.log_probs[row.index * K + k];
     Tm::sync();
-    merge_list<kThreads>(p, idx, K);
+    merge_list<kThreads>(p, idx, seen, K);
     if (Tm::warp() < list_warps) {
       const ListSums ls = list_sums(p, zu, idx, K, Tm::tid(), 32 * list_warps, o.renormalize, inv_t);
       if (Tm::lane() == 0) lred[slot][Tm::warp()] = ls;

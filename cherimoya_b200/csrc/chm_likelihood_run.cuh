@@ -24,13 +24,13 @@ int largest(const Rows& a) { return *std::max_element(a.size, a.size + a.ng); }
 // Distillation with a gradient keeps a block's share of a row in shared memory
 // from the first look to the last, so the row's size sets how many blocks an
 // SM holds. A warp takes a short row and a block of 128 one of up to 44 KB, of
-// which five fit: 8,192 x 20,000 bf16 entries take 147 us with it and 185 with
-// 256 threads, 8,192 x 9,000 take 108 and 150; 8,192 x 32,768, of which
-// three fit, take 220 with 256 threads, 267 with 128 and 326 with 512, which
-// only rows above that get. Rows of more than kChunkBytes are shared by the
-// blocks of a cluster, so that each holds its share; few long rows are cut
-// further, to reach more SMs. Many rows are not (8,192 x 32,768 in clusters of
-// two: 387 us).
+// which five fit: 8,192 x 20,000 bf16 entries take 151 us with it and 185 with
+// 256 threads, 8,192 x 9,000 take 92 and 150. Above that it is a block of 256:
+// 8,192 x 32,768 entries, of which three rows fit, take 220 us, 267 with 128
+// threads and 326 with 512; 2,048 x 40,000, of which two fit, 101 and with 512
+// 155. Rows of more than kChunkBytes are shared by the blocks of a cluster, so
+// that each holds its share; few long rows are cut further, to reach more SMs.
+// Many rows are not (8,192 x 32,768 in clusters of two: 387 us).
 constexpr int kChunkBytes = 96 << 10;
 Cut cut_rows(int nvec, long long rows, bool warp) {
   Cut c{};
@@ -38,8 +38,8 @@ Cut cut_rows(int nvec, long long rows, bool warp) {
   while (c.log_blocks < 3 && rows << c.log_blocks < 2 * 148 && nvec > 512 << c.log_blocks)
     ++c.log_blocks;
   const int share = (nvec + (1 << c.log_blocks) - 1) >> c.log_blocks;
-  c.threads = warp && share <= 256 ? 32 : share <= 2816 ? 128 : share <= 4096 ? 256 : 512;
-  if (c.log_blocks && c.threads < 256) c.threads = 256;
+  c.threads = warp && share <= 256 ? 32 : share <= 2816 ? 128 : 256;
+  if (c.log_blocks && c.threads < 128) c.threads = 128;
   const int most = std::min(std::max(share, 1), kChunkBytes / 16);
   c.cap = (most + kBatch * c.threads - 1) / (kBatch * c.threads) * (kBatch * c.threads);
   return c;
@@ -137,7 +137,7 @@ int run_log_probs_grad_m(const Rows& a, const ScoreGradArgs& o, long long n, cud
   int log_blocks = 0;
   while (threads == 256 && nvec > 4096 << log_blocks) ++log_blocks;
   const int spots = o.n_targets * (o.g_log_probs != nullptr) + o.top_k * (o.g_top != nullptr);
-  const size_t smem = (size_t)(threads == 32 ? 4 : 1) * spots * 8;
+  const size_t smem = (size_t)(threads == 32 ? 4 : 1) * (sort_size(spots) + spots) * 4;
   auto run = [&](auto kernel) {
     return launch(kernel, threads, log_blocks, n, smem, st, false, a, o, (unsigned)n,
                   log_blocks);
@@ -176,8 +176,7 @@ int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t
   switch (c.threads) {
     case 32: return run(distill_kernel<T, 32, kMask>);
     case 128: return run(distill_kernel<T, 128, kMask>);
-    case 256: return run(distill_kernel<T, 256, kMask>);
-    default: return run(distill_kernel<T, 512, kMask>);
+    default: return run(distill_kernel<T, 256, kMask>);
   }
 }
 
