@@ -195,7 +195,7 @@ int32_t chm_variant(const chm_model_desc* desc, const void* packed, int32_t n_pa
  * of z / temperature over the entries that take part. A row with none has the
  * normaliser -inf, the entropy 0, loss 0 and gradient 0; a row with NaN or
  * +inf among them has no distribution and answers NaN.
- * Neither call needs a workspace; every call can be captured in a graph. */
+ * No call needs a workspace, and every call can be captured in a graph. */
 typedef enum { CHM_LOGITS_F32 = 0, CHM_LOGITS_BF16 = 1, CHM_LOGITS_F16 = 2 } chm_logits_dtype;
 
 #define CHM_ROW_MAX_ENTRIES (1 << 20) /* entries of one row              */

@@ -124,3 +124,27 @@ def test_many_targets():
 @pytest.mark.parametrize("dtype", [K.F32, K.F16])
 def test_temperatures(dtype, T):
     K.case_temperatures(DEV, dtype, T)
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_launches_on_the_logits_device(monkeypatch, current):
+    """The call runs with the logits' device current, on that device's stream, whichever device
+    was current, and that one is current again behind it."""
+    from cherimoya_b200 import ops
+    state = {"current": current}
+
+    class Guard:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, state["current"] = state["current"], self.index
+
+        def __exit__(self, *_):
+            state["current"] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    seen = ops._on(torch.device("cuda", 1), lambda *a: (state["current"],) + a, "x")
+    assert seen == (1, "x", 101) and state["current"] == current
