@@ -1355,8 +1355,8 @@ __device__ __noinline__ void merge_list(double* p, int* idx, uint32_t* key, int 
 // slots 132; with three blocks to an SM one loads while another computes, but
 // not all the time. A block that went from row to row and asked for the next
 // early took 255. Without a gradient 1,024 x 100,003 fp32 with 100 listed take
-// 96 us, 4.3 TB/s: 1.4 rounds of blocks. 1,024 x 1,000 fp32 with 32 listed take
-// 9 us, which is the latency of one row.
+// 85 us, 4.9 TB/s; every row has a block at once, and with it the barriers of its
+// chunks. 1,024 x 1,000 fp32 with 32 listed take 9 us, the latency of one row.
 // At least three blocks of 256 to an SM, which 64 KB of shared memory allow, and
 // seven of 128.
 template <typename T, int kThreads, bool kMask>

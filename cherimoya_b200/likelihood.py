@@ -208,8 +208,8 @@ def _cpu_log_probs_backward(logits, mask, groups, targets, top_indices, stats, e
     z, sizes = _cpu_rows(logits, mask, groups)
     R = z.shape[0]
     m, log_s = stats[:, :1], stats[:, 1:]
-    lists = [(i.reshape(R, i.shape[-1]), g.reshape(R, i.shape[-1])) for i, g in ((targets, g_lp), (top_indices, g_top))
-             if g is not None]
+    lists = [(i.reshape(R, i.shape[-1]), g.reshape(R, i.shape[-1]))
+             for i, g in ((targets, g_lp), (top_indices, g_top)) if g is not None]
     idx = torch.cat([i for i, _ in lists], -1) if lists else torch.empty(R, 0, dtype=torch.int64)
     g = torch.cat([x for _, x in lists], -1) if lists else torch.empty(R, 0)
     zt, past = _cpu_gather(z, idx, sizes)
