@@ -162,7 +162,7 @@ int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t
     // Without a gradient nothing is looked at twice, so a block of 128 takes
     // chunks of 8 KB, the next on its way while it sums one, and seven blocks fit
     // an SM: 1,024 x 100,003 fp32 entries take 85 us (16 KB: 95; 32 KB and 256
-    // threads: 118), 2,048 x 100,003 bf16 93 (103; 118), 4,096 x 25,000 fp32 83
+    // threads: 96), 2,048 x 100,003 bf16 93 (103; 118), 4,096 x 25,000 fp32 83
     // (84; 104), 8,192 x 12,000 bf16 79 (held whole: 120). Below 16 KB a row is
     // one chunk. Few rows are cut until there are three blocks to an SM.
     c = {128, 0, 512};
