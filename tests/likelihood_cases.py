@@ -474,3 +474,24 @@ def case_temperatures(dev, dtype, T):
     loss, grad = cb.distillation_loss_and_grad(z[::2], idx[::2], lp[::2] - 0.1, temperature=T,
                                                reduction="none")
     C.check_distill(z[::2], idx[::2], lp[::2] - 0.1, False, None, None, T, None, "none", loss, grad)
+
+
+def case_ends(dev, dtype, v, k, rows):
+    """Some of a row's first and last entries, which no full vector holds, are listed and some not."""
+    z, g = C.logits((rows, v), dtype, v + k)
+    z[:, [0, 2, -1, -3]] += 4.0
+    idx = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(rows)])
+    ends = torch.tensor([0, 1, 4, 6, v - 1, v - 2, v - 4, v - 7])
+    inner = (idx > 7) & (idx < v - 8)
+    idx = torch.where(inner, idx, -1)
+    at = torch.randperm(k, generator=g)[:8]
+    for r in range(rows):
+        idx[r, at] = ends.roll(r) if r % 3 else torch.where(ends % 2 == r % 2, ends, -1)
+    lp = torch.log_softmax(torch.randn(rows, k, generator=g), -1) - 0.3
+    z, idx, lp = z.to(dev), idx.to(dev), lp.to(dev)
+    for renorm in (False, True):
+        how = dict(renormalize=renorm, reduction="none")
+        loss, grad = cb.distillation_loss_and_grad(z, idx, lp, **how)
+        C.check_distill(z, idx, lp, renorm, None, None, 1.0, None, "none", loss, grad)
+        C.check_distill(z, idx, lp, renorm, None, None, 1.0, None, "none",
+                        cb.distillation_loss(z, idx, lp, **how), None)

@@ -336,3 +336,10 @@ def test_windows_and_masks_off_their_boundaries(dtype):
             lp = out.top_log_probs.detach() - 0.1
             loss, grad = cb.distillation_loss_and_grad(z, out.top_indices, lp, mask=m)
             C.check_distill(z, out.top_indices, lp, False, m, None, 1.0, None, "mean", loss, grad)
+
+
+@pytest.mark.parametrize("v,k,rows", [(61, 9, 9), (1003, 40, 9), (1003, 200, 9), (9005, 50, 9),
+                                      (9005, 50, 600), (20011, 300, 600), (100003, 40, 5)])
+@pytest.mark.parametrize("dtype", [K.F32, K.BF16, K.F16])
+def test_ends(dtype, v, k, rows):
+    K.case_ends(DEV, dtype, v, k, rows)

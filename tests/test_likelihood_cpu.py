@@ -148,3 +148,8 @@ def test_launches_on_the_logits_device(monkeypatch, current):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
     seen = ops._on(torch.device("cuda", 1), lambda *a: (state["current"],) + a, "x")
     assert seen == (1, "x", 101) and state["current"] == current
+
+
+@pytest.mark.parametrize("dtype", [K.F32, K.BF16])
+def test_ends(dtype):
+    K.case_ends(DEV, dtype, 131, 40, 5)
