@@ -576,7 +576,8 @@ template <int kThreads> struct TopShared {
   uint4 hold[Team<kThreads>::kWarps][32];
   int hold_at[Team<kThreads>::kWarps][32];
   uint8_t list[Team<kThreads>::kWarps][32 * kBatch];
-  int count;
+  int count;                       // candidates found; written no more once the team has read it
+  int kept;                        // what thin_out or count_top leaves of them
   int red[Team<kThreads>::kWarps];
 };
 
@@ -625,14 +626,14 @@ __device__ __noinline__ int count_top(const Row<T>& row, const Share<T>& share, 
     if (count(lo, true, mid) >= need) last = mid; else before = mid;
   }
   Tm::sync();
-  if (Tm::tid() == 0) sh.count = 0;
+  if (Tm::tid() == 0) sh.kept = 0;
   Tm::sync();
   each_entry<T, kThreads, kMask>(row, share, edge, [&](float z, int v) {
     const uint32_t key = logit_key(z);
-    if (key > lo || (key == lo && v <= last)) sh.cand[atomicAdd(&sh.count, 1)] = order_key(key, v);
+    if (key > lo || (key == lo && v <= last)) sh.cand[atomicAdd(&sh.kept, 1)] = order_key(key, v);
   });
   Tm::sync();
-  return sh.count;
+  return sh.kept;
 }
 
 // Drops candidates that are too many to be ranked one against all: the first
@@ -666,10 +667,10 @@ __device__ __noinline__ int thin_out(int n, int k, TopShared<kThreads>& sh) {
       kept += __popc(vote);
       __syncwarp();
     }
-    if (lane == 0) sh.count = kept;
+    if (lane == 0) sh.kept = kept;
   }
   Tm::sync();
-  return sh.count;
+  return sh.kept;
 }
 
 // The k largest entries of a block's share and some more, in no order, into
@@ -849,7 +850,7 @@ __device__ __forceinline__ int collect_top(const Row<T>& row, const Share<T>& sh
     if (at < TopShared<kThreads>::kMaxCand) sh.cand[at] = order_key(logit_key(edge), share.edge);
   }
   Tm::sync();
-  const int n = sh.count;
+  const int n = sh.count;                              // every thread takes the same way from here
   if (n <= 2 * k + 16) return n;
   if (n <= TopShared<kThreads>::kMaxCand) return thin_out<kThreads>(n, k, sh);
   return count_top<T, kThreads, kMask>(row, share, edge, lo, k, sh);
