@@ -1347,7 +1347,8 @@ __device__ __noinline__ void merge_list(double* p, int* idx, uint32_t* key, int 
 // the two normalisers and q_R = exp(lse_R - lse)
 //   dz_v = T w exp(z'_v - lse_R) (q_R - P_rest)     outside the list
 //   dz_u = T w (exp(z'_u - lse) - P_u)              in it
-// so the gradient is one more exponential per entry in shared memory. Without
+// so the gradient is one more exponential per entry in shared memory, and
+// q_R - P_rest = P_list - q_list where the rest has most of the mass. Without
 // a gradient the chunks are small and there are two, one on its way.
 // The first warps add up the list while the others begin with the row.
 //
@@ -1546,8 +1547,12 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
   // the two normalisers relative to the larger of the two maxima
   const float big = fmaxf(rest ? sum.m : neg_inf(), ls.top_z);
   const float norm_r = rest ? sum.s * ex2((sum.m - big) * a.c) : 0.f;
-  const float inv_norm =
-      __fdividef(1.f, norm_r + (listed ? ls.e * ex2((ls.top_z - big) * a.c) : 0.f));
+  const float norm_u = listed ? ls.e * ex2((ls.top_z - big) * a.c) : 0.f;
+  const float inv_norm = __fdividef(1.f, norm_r + norm_u);
+  // q_R - P_rest, from the complements where those are the smaller numbers: as the difference
+  // of two numbers near 1 it would keep no digits of a list with little mass
+  const float over =
+      p_r > 0.5f ? (float)ls.mass - norm_u * inv_norm : norm_r * inv_norm - p_r;
   const float scaled = weight * o.scale *
                        (o.upstream ? o.upstream[row.index * o.upstream_stride] : 1.f);
   // by the last warp, when the others are done; a function call to a lane
@@ -1579,7 +1584,7 @@ distill_kernel(const __grid_constant__ Rows a, const DistillArgs o, unsigned row
     return;
   }
   const float scale = live ? scaled * a.t : 0.f, ref = rest ? sum.m : 0.f;
-  const float coef = live && rest ? __fdividef(scale * (norm_r * inv_norm - p_r), sum.s) : 0.f;
+  const float coef = live && rest ? __fdividef(scale * over, sum.s) : 0.f;
   const float nan = bad || coef != coef ? quiet_nan() : 0.f;   // of a row without a distribution
   const float2 nref = {-ref, -ref}, cc = {a.c, a.c}, kk = {coef, coef};
   auto slope = [&](const uint4& r, int j) {

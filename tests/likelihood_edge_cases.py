@@ -28,3 +28,36 @@ def case_candidates(dev, dtype, v, rows):
         for _ in range(3):
             out = cb.profile_log_probs(z, t, top_k=k)
         C.check_scores(z, out, t, k, None, None, 1.0)
+
+
+def case_small_mass(dev, dtype, v, k, rows):
+    """Lists of little mass: outside the list the gradient is the entry's share of the rest times
+    (list's mass under the teacher - its mass under the student), and its error is bounded by
+    those two masses, not by the rest's, which are nearly 1. From the bounds of
+    likelihood_common.py each mass is off by at most 2 CHAIN U of itself, and so is the share.
+    Without a list the gradient is exactly 0."""
+    g = torch.Generator().manual_seed(v + k)
+    z = (0.5 * torch.randn(rows, v, generator=g)).to(dtype)
+    q = torch.log_softmax(z.double(), -1)
+    idx = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(rows)])
+    lp = (q.gather(-1, idx) + 0.3 * torch.randn(rows, k, generator=g)).float()
+    loss, grad = cb.distillation_loss_and_grad(z.to(dev), idx.to(dev), lp.to(dev),
+                                               reduction="none")
+    listed = torch.zeros(rows, v, dtype=torch.bool).scatter_(-1, idx, True)
+    p_u, q_u = lp.double().exp(), q.gather(-1, idx).exp()
+    p_list, q_list = p_u.sum(-1, keepdim=True), q_u.sum(-1, keepdim=True)
+    assert float(p_list.max()) < 0.5 and float(q_list.max()) < 0.5
+    share = torch.where(listed, 0.0, q.exp() / (1 - q_list))
+    want = share * (p_list - q_list)
+    want.scatter_(-1, idx, q_u - p_u)
+    mag = share * (p_list + q_list)
+    mag.scatter_(-1, idx, q_u + p_u)
+    tol = C.HALF_STEP[dtype] * want.abs() + 2 * C.CHAIN * C.U * mag + C.TINY[dtype]
+    C.same(grad, want, tol, "gradient")
+    z = z.to(dev).requires_grad_()
+    loss = cb.distillation_loss(z, idx.to(dev), lp.to(dev), reduction="sum")
+    auto, = torch.autograd.grad(loss, z)
+    C.same(auto, want, tol, "gradient through autograd")
+    none = torch.empty(rows, 0, device=dev)
+    loss, grad = cb.distillation_loss_and_grad(z, none.long(), none)
+    assert float(loss) == 0.0 and float(grad.abs().max()) == 0.0

@@ -19,3 +19,11 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_candidates(dtype, v, rows):
     E.case_candidates(DEV, dtype, v, rows)
+
+
+# a warp, blocks of 128 and 256 and a cluster to a row
+@pytest.mark.parametrize("v,k,rows", [(300, 1, 9), (1000, 7, 9), (1000, 200, 9), (9001, 5, 9),
+                                      (32768, 1, 400), (32768, 64, 400), (200003, 3, 3)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_small_mass(dtype, v, k, rows):
+    E.case_small_mass(DEV, dtype, v, k, rows)

@@ -17,3 +17,9 @@ F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_candidates(dtype):
     E.case_candidates(DEV, dtype, 5003, 3)
+
+
+@pytest.mark.parametrize("v,k", [(700, 1), (30001, 5)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_small_mass(dtype, v, k):
+    E.case_small_mass(DEV, dtype, v, k, 4)
