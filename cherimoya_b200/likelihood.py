@@ -35,6 +35,7 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .model import _validate_signal_groups
@@ -57,6 +58,22 @@ class ProfileLogProbs(NamedTuple):
 
 def _fail(text):
     raise RuntimeError("cherimoya_b200: " + text)
+
+
+_compiled = torch.compiler.is_compiling
+_transforms = torch._C._are_functorch_transforms_active
+
+
+def _check_reverse(t, name):
+    """Refuses tangents of forward mode and the tensors of torch.func's transforms: the formulas
+    run on the tensor's memory and would drop them without a word. A tensor that is traced shows
+    neither, so there an open dual level or an active transform is refused."""
+    if forward_ad._current_level < 0 and not _transforms():
+        return
+    if _compiled() or torch._C._functorch.is_functorch_wrapped_tensor(t) or \
+            forward_ad.unpack_dual(t).tangent is not None:
+        _fail("{} must be a plain tensor: forward-mode derivatives and torch.func transforms are "
+              "not supported".format(name))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -85,6 +102,7 @@ def _check(logits, mask, signal_groups, temperature):
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
         _fail("logits must be a float32, bfloat16 or float16 tensor, got {}".format(
             getattr(logits, "dtype", type(logits).__name__)))
+    _check_reverse(logits, "logits")
     groups = None if signal_groups is None else tuple(signal_groups)
     lead = _check_shape(logits.shape, groups)
     if not _MIN_T <= temperature <= _MAX_T:
@@ -291,9 +309,6 @@ def _cpu_distill(logits, mask, groups, idx, t_lp, renormalize, weight, scale, up
 
 
 # ------------------------------------------------------------ dispatch
-_compiled = torch.compiler.is_compiling
-
-
 def _run_log_probs(logits, mask, groups, lead, targets, top_k, temperature, want_stats):
     if logits.is_cuda:
         from . import ops
@@ -344,7 +359,8 @@ def profile_log_probs(logits, targets=None, *, top_k=0, mask=None, signal_groups
     -inf and index -1. temperature divides the logits.
 
     Returns ``ProfileLogProbs``; all but ``top_indices`` are differentiable
-    with respect to the logits (once).
+    with respect to the logits (once, in reverse mode; forward mode and the
+    transforms of ``torch.func`` are refused).
     """
     groups, mask, lead = _check(logits, mask, signal_groups, temperature)
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= MAX_TOP:
@@ -423,6 +439,7 @@ def _constant(t, name, device):
     """t in fp32 and contiguous; it carries no gradient."""
     if t.device != device:
         _fail("{} must be on the logits' device".format(name))
+    _check_reverse(t, name)
     if t.requires_grad:
         if torch.is_grad_enabled():
             _fail("{} takes no gradient: detach it".format(name))
@@ -452,7 +469,8 @@ def distillation_loss(logits, teacher_indices, teacher_log_probs, *, renormalize
 
     weight (lead): a factor per row; a row of weight 0 is not looked at.
     reduction: 'mean' over all rows, 'sum', or 'none' (lead). The result is
-    fp32 and differentiable with respect to the logits (once).
+    fp32 and differentiable with respect to the logits (once, in reverse mode;
+    forward mode and the transforms of ``torch.func`` are refused).
     """
     groups, mask, lead, idx, t_lp, weight, scale = _check_distill(
         logits, teacher_indices, teacher_log_probs, mask, signal_groups, temperature, weight,

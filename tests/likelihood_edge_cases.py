@@ -1,5 +1,6 @@
 """More cases of the likelihood and distillation tests, run on the device they are given."""
 
+import pytest
 import torch
 
 import cherimoya_b200 as cb
@@ -61,3 +62,55 @@ def case_small_mass(dev, dtype, v, k, rows):
     none = torch.empty(rows, 0, device=dev)
     loss, grad = cb.distillation_loss_and_grad(z, none.long(), none)
     assert float(loss) == 0.0 and float(grad.abs().max()) == 0.0
+
+
+def _calls():
+    """(what is transformed, function of it) of every public call and every differentiable-looking
+    argument; the others are plain."""
+    g = torch.Generator().manual_seed(2)
+    z, idx = torch.randn(3, 20, generator=g), torch.randint(0, 20, (3, 4), generator=g)
+    lp, w = torch.full((3, 4), -2.0), torch.ones(3)
+    return {
+        "scores": (z, lambda d, x: cb.profile_log_probs(x, top_k=2).entropy.sum()),
+        "loss": (z, lambda d, x: cb.distillation_loss(x, idx.to(d), lp.to(d))),
+        "loss and grad": (z, lambda d, x: cb.distillation_loss_and_grad(x, idx.to(d),
+                                                                        lp.to(d))[0]),
+        "teacher": (lp, lambda d, x: cb.distillation_loss(z.to(d), idx.to(d), x)),
+        "weight": (w, lambda d, x: cb.distillation_loss(z.to(d), idx.to(d), lp.to(d), weight=x)),
+    }
+
+
+CALLS = sorted(_calls())
+
+
+def _dual(f, x):
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        return forward_ad.unpack_dual(f(forward_ad.make_dual(x, torch.ones_like(x)))).tangent
+
+
+TRANSFORMS = {
+    "jvp": lambda f, x: torch.func.jvp(f, (x,), (x,)),
+    "jacfwd": lambda f, x: torch.func.jacfwd(f)(x),
+    "grad": lambda f, x: torch.func.grad(f)(x),
+    "vmap": lambda f, x: torch.func.vmap(f)(x[None]),
+    "dual": _dual,
+    "dual without grad": torch.no_grad()(_dual),
+    "dual that requires grad": lambda f, x: _dual(f, x.clone().requires_grad_()),
+}
+
+
+def case_transforms(dev, call, transform):
+    """Derivatives that the calls do not form are refused, never 0."""
+    x, f = _calls()[call]
+    with pytest.raises(RuntimeError, match="forward-mode|takes no gradient"):
+        TRANSFORMS[transform](lambda v: f(dev, v), x.to(dev))
+    assert torch.isfinite(f(dev, x.to(dev))).all()           # and a plain call works behind it
+
+
+def case_beside_forward_mode(dev):
+    """Plain tensors, a fixed teacher's, are scored while others carry tangents."""
+    z = torch.linspace(-1, 1, 20, device=dev).repeat(3, 1)
+    want = cb.profile_log_probs(z).entropy.sum()
+    got = _dual(lambda x: cb.profile_log_probs(z).entropy.sum() * x, torch.tensor(2.0, device=dev))
+    assert torch.equal(got, want)

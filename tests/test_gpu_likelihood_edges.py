@@ -27,3 +27,13 @@ def test_candidates(dtype, v, rows):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_small_mass(dtype, v, k, rows):
     E.case_small_mass(DEV, dtype, v, k, rows)
+
+
+@pytest.mark.parametrize("transform", sorted(E.TRANSFORMS))
+@pytest.mark.parametrize("call", E.CALLS)
+def test_transforms(call, transform):
+    E.case_transforms(DEV, call, transform)
+
+
+def test_beside_forward_mode():
+    E.case_beside_forward_mode(DEV)

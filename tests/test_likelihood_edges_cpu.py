@@ -23,3 +23,29 @@ def test_candidates(dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_small_mass(dtype, v, k):
     E.case_small_mass(DEV, dtype, v, k, 4)
+
+
+@pytest.mark.parametrize("transform", sorted(E.TRANSFORMS))
+@pytest.mark.parametrize("call", E.CALLS)
+def test_transforms(call, transform):
+    E.case_transforms(DEV, call, transform)
+
+
+def test_beside_forward_mode():
+    E.case_beside_forward_mode(DEV)
+
+
+@pytest.mark.parametrize("transform", ["grad", "jvp", "vmap", "dual"])
+@pytest.mark.parametrize("call", ["scores", "loss and grad"])
+def test_transforms_while_tracing(call, transform):
+    """Inside a compiled function and around one."""
+    x, f = E._calls()[call]
+    t = E.TRANSFORMS[transform]
+    torch._dynamo.reset()
+    inside = torch.compile(lambda v: t(lambda u: f(DEV, u), v), backend="eager")
+    compiled = torch.compile(lambda v: f(DEV, v), backend="eager")
+    assert torch.isfinite(compiled(x)).all()
+    for run in (inside, lambda v: t(compiled, v)):
+        with pytest.raises(Exception, match="forward-mode"):
+            run(x)
+    torch._dynamo.reset()
