@@ -76,6 +76,12 @@ def _check_reverse(t, name):
               "not supported".format(name))
 
 
+def _check_constant(t, name):
+    _check_reverse(t, name)
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail("{} takes no gradient: detach it".format(name))
+
+
 @functools.lru_cache(maxsize=1024)
 def _check_shape(shape, groups):
     """The shape of the per-row results; groups: None, or a tuple."""
@@ -98,13 +104,17 @@ def _check_shape(shape, groups):
 
 
 def _check(logits, mask, signal_groups, temperature):
-    """(groups as a tuple, empty for none; the mask in the logits' shape; the rows' shape)"""
+    """(groups as a tuple, empty for none; the mask in the logits' shape; the rows' shape; the
+    temperature as a number)"""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES:
         _fail("logits must be a float32, bfloat16 or float16 tensor, got {}".format(
             getattr(logits, "dtype", type(logits).__name__)))
     _check_reverse(logits, "logits")
     groups = None if signal_groups is None else tuple(signal_groups)
     lead = _check_shape(logits.shape, groups)
+    if isinstance(temperature, torch.Tensor):
+        _check_constant(temperature, "temperature")
+        temperature = float(temperature.detach())
     if not _MIN_T <= temperature <= _MAX_T:
         raise ValueError("temperature must be between 1/1024 and 1024, got {!r}".format(
             temperature))
@@ -119,7 +129,7 @@ def _check(logits, mask, signal_groups, temperature):
             except RuntimeError:
                 _fail("mask of shape {} does not broadcast to the logits' {}".format(
                     tuple(mask.shape), tuple(logits.shape)))
-    return groups or (), mask, lead
+    return groups or (), mask, lead, temperature
 
 
 def _check_list(t, name, lead, device):
@@ -356,13 +366,13 @@ def profile_log_probs(logits, targets=None, *, top_k=0, mask=None, signal_groups
     probability 0, no gradient), one past the row answers NaN, a cell that
     does not take part -inf (no gradient). top_k: up to 128 cells, the most
     likely first, equal logits by ascending index; places without a cell hold
-    -inf and index -1. temperature divides the logits.
+    -inf and index -1. temperature, a number, divides the logits.
 
     Returns ``ProfileLogProbs``; all but ``top_indices`` are differentiable
     with respect to the logits (once, in reverse mode; forward mode and the
     transforms of ``torch.func`` are refused).
     """
-    groups, mask, lead = _check(logits, mask, signal_groups, temperature)
+    groups, mask, lead, temperature = _check(logits, mask, signal_groups, temperature)
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= MAX_TOP:
         raise ValueError("top_k must be an int between 0 and {}, got {!r}".format(MAX_TOP, top_k))
     if targets is None:
@@ -414,7 +424,7 @@ class _Distill(torch.autograd.Function):
 
 def _check_distill(logits, indices, log_probs, mask, signal_groups, temperature, weight,
                    reduction):
-    groups, mask, lead = _check(logits, mask, signal_groups, temperature)
+    groups, mask, lead, temperature = _check(logits, mask, signal_groups, temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got {!r}".format(reduction))
     device = logits.device
@@ -432,17 +442,15 @@ def _check_distill(logits, indices, log_probs, mask, signal_groups, temperature,
     for extent in lead:
         rows *= extent
     scale = 1.0 / rows if reduction == "mean" and rows else 1.0
-    return groups, mask, lead, indices, log_probs, weight, scale
+    return groups, mask, lead, temperature, indices, log_probs, weight, scale
 
 
 def _constant(t, name, device):
     """t in fp32 and contiguous; it carries no gradient."""
     if t.device != device:
         _fail("{} must be on the logits' device".format(name))
-    _check_reverse(t, name)
+    _check_constant(t, name)
     if t.requires_grad:
-        if torch.is_grad_enabled():
-            _fail("{} takes no gradient: detach it".format(name))
         t = t.detach()
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
@@ -472,7 +480,7 @@ def distillation_loss(logits, teacher_indices, teacher_log_probs, *, renormalize
     fp32 and differentiable with respect to the logits (once, in reverse mode;
     forward mode and the transforms of ``torch.func`` are refused).
     """
-    groups, mask, lead, idx, t_lp, weight, scale = _check_distill(
+    groups, mask, lead, temperature, idx, t_lp, weight, scale = _check_distill(
         logits, teacher_indices, teacher_log_probs, mask, signal_groups, temperature, weight,
         reduction)
     reduce, renormalize = reduction != "none", bool(renormalize)
@@ -494,7 +502,7 @@ def distillation_loss_and_grad(logits, teacher_indices, teacher_log_probs, *, re
     that of the losses' sum. Neither carries an autograd graph: continue with
     ``logits.backward(grad)``. What multiplies the loss goes into ``weight``.
     """
-    groups, mask, lead, idx, t_lp, weight, scale = _check_distill(
+    groups, mask, lead, temperature, idx, t_lp, weight, scale = _check_distill(
         logits, teacher_indices, teacher_log_probs, mask, signal_groups, temperature, weight,
         reduction)
     reduce = reduction != "none"

@@ -114,3 +114,28 @@ def case_beside_forward_mode(dev):
     want = cb.profile_log_probs(z).entropy.sum()
     got = _dual(lambda x: cb.profile_log_probs(z).entropy.sum() * x, torch.tensor(2.0, device=dev))
     assert torch.equal(got, want)
+
+
+def case_temperature_is_a_number(dev):
+    """A tensor's value counts, its gradient would be lost: it is refused."""
+    z = torch.linspace(-1, 1, 20, device=dev).repeat(3, 1)
+    idx, lp = torch.zeros(3, 1, dtype=torch.int64, device=dev), torch.full((3, 1), -1.0, device=dev)
+    learnt = torch.tensor(2.0, device=dev, requires_grad=True)
+    calls = [lambda x, T: cb.profile_log_probs(x, top_k=2, temperature=T)[1:4],
+             lambda x, T: (cb.distillation_loss(x, idx, lp, temperature=T),),
+             lambda x, T: cb.distillation_loss_and_grad(x, idx, lp, temperature=T)]
+    for call in calls:
+        for x in (z, z.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="temperature takes no gradient"):
+                call(x, learnt)
+            want = call(x, 2.0)
+            for T in (learnt.detach(), learnt.detach().cpu().double()):
+                got = call(x, T)
+                assert all(torch.equal(a, b) and a.requires_grad == b.requires_grad
+                           for a, b in zip(got, want))
+            with torch.no_grad():
+                assert all(torch.equal(a, b) for a, b in zip(call(x, learnt), want))
+        with pytest.raises(RuntimeError, match="temperature must be a plain tensor"):
+            _dual(lambda T: call(z, T)[0], learnt.detach())
+        with pytest.raises(ValueError, match="temperature"):
+            call(z, torch.tensor(0.0, device=dev))

@@ -37,3 +37,7 @@ def test_transforms(call, transform):
 
 def test_beside_forward_mode():
     E.case_beside_forward_mode(DEV)
+
+
+def test_temperature_is_a_number():
+    E.case_temperature_is_a_number(DEV)

@@ -49,3 +49,7 @@ def test_transforms_while_tracing(call, transform):
         with pytest.raises(Exception, match="forward-mode"):
             run(x)
     torch._dynamo.reset()
+
+
+def test_temperature_is_a_number():
+    E.case_temperature_is_a_number(DEV)
