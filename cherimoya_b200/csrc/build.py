@@ -21,7 +21,7 @@ SOURCES = [os.path.join(HERE, f) for f in (
     "chm_likelihood_f16.cu")]
 DEPS = SOURCES + [os.path.join(HERE, f) for f in (
     "chm_kernels.cuh", "chm_likelihood.cuh", "chm_likelihood_run.cuh", "chm_likelihood.h",
-    "chm_host.h", "chm_ptx.cuh")] + [
+    "chm_exp64.h", "chm_host.h", "chm_ptx.cuh")] + [
     os.path.join(ROOT, "include", "cherimoya_b200.h")]
 
 

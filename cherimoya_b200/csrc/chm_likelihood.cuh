@@ -10,6 +10,7 @@
 
 #include <cstdint>
 
+#include "chm_exp64.h"
 #include "chm_likelihood.h"
 #include "chm_ptx.cuh"
 
@@ -1217,24 +1218,6 @@ template <typename T> __device__ __forceinline__ void sts_neg_inf(uint32_t a) {
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(Vec<T>::kNegInf) : "memory");
   else
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((uint16_t)Vec<T>::kNegInf) : "memory");
-}
-
-// exp in 64 bits, for masses that are added up and taken from 1: x = n log 2 + r
-// with |r| <= log(2) / 2, and the Taylor sum of e^r to r^11 (the rest is below
-// 7e-15) in a tree, since one call after the other waits for fp64's latency.
-// 0 below -700, where no mass is left; inf above 700.
-__device__ __forceinline__ double exp64(double x) {
-  const double n = rint(x * 1.4426950408889634);
-  const double r = fma(n, -1.9082149292705877e-10, fma(n, -6.9314718036912382e-1, x));
-  const double r2 = r * r, r4 = r2 * r2;
-  const double a = fma(fma(1.0 / 6, r, 0.5), r2, 1.0 + r);
-  const double b = fma(fma(1.0 / 5040, r, 1.0 / 720), r2, fma(1.0 / 120, r, 1.0 / 24));
-  const double c = fma(fma(1.0 / 39916800, r, 1.0 / 3628800), r2,
-                       fma(1.0 / 362880, r, 1.0 / 40320));
-  const double e = fma(fma(c, r4, b), r4, a);
-  const int k = (int)fmin(fmax(n, -1010.0), 1010.0);
-  const double s = e * __hiloint2double((1023 + k) << 20, 0);
-  return x < -700.0 ? 0.0 : x > 700.0 ? (double)__int_as_float(0x7f800000) : s;
 }
 
 // Per warp: what the list adds up to.
