@@ -50,12 +50,15 @@ Cut cut_rows(int nvec, long long rows, bool warp) {
 // masked fp32 entries take 50 us, 56 with teams of 64 and 79 with 128. Longer rows get
 // a block of 128 (4,096 x 50,001 bf16: 88 us, 109 with 256), more than 64 top
 // entries too, since a lane keeps at most two; few long rows are shared by the
-// blocks of a cluster.
+// blocks of a cluster, and so are rows of which a thread would add up more than
+// kMaxBatches batches one by one.
 Cut cut_stream(int nvec, long long rows, int top_k) {
   Cut c{};
   c.threads = nvec <= 512 && top_k <= 64 ? 32 : 128;
   if (c.threads == 128)
-    while (c.log_blocks < 3 && rows << c.log_blocks < 6 * 148 && nvec > 1024 << c.log_blocks)
+    while (c.log_blocks < 3 &&
+           ((rows << c.log_blocks < 6 * 148 && nvec > 1024 << c.log_blocks) ||
+            nvec > kMaxBatches * kBatch * 128 << c.log_blocks))
       ++c.log_blocks;
   return c;
 }
@@ -176,9 +179,12 @@ int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t
     return launch(kernel, c.threads, c.log_blocks, n, smem, st, true, a, o, (unsigned)n,
                   c.log_blocks, c.cap, chunks, team);
   };
+  // a chunk is a batch per thread
+  const bool many = chunks > 1 && nvec > kMaxBatches * c.cap << c.log_blocks;
   switch (c.threads) {
     case 32: return run(distill_kernel<T, 32, kMask>);
-    case 128: return run(distill_kernel<T, 128, kMask>);
+    case 128: return many ? run(distill_kernel<T, 128, kMask, true>)
+                          : run(distill_kernel<T, 128, kMask>);
     default: return run(distill_kernel<T, 256, kMask>);
   }
 }

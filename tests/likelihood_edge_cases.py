@@ -1,5 +1,7 @@
 """More cases of the likelihood and distillation tests, run on the device they are given."""
 
+import math
+
 import pytest
 import torch
 
@@ -139,3 +141,41 @@ def case_temperature_is_a_number(dev):
             _dual(lambda T: call(z, T)[0], learnt.detach())
         with pytest.raises(ValueError, match="temperature"):
             call(z, torch.tensor(0.0, device=dev))
+
+
+def case_long_sums(dev, dtype, rows, every):
+    """Rows of 2^20 entries that are nearly all alike, so that the roundings of a sum have one
+    sign: every 509th entry, and so some that every thread has, is 0 and the others have a value
+    between -0.69 and 0, different from row to row; with `every`, each entry of that multiple is
+    -inf. With |x| <= 0.7 a term is off by (4 + 3 * 0.7) U of itself, the sum by 80 U more (partial
+    sums of at most 64 terms in a row and 16 joins, as likelihood_common.py has it), and its
+    logarithm by 2 U of itself."""
+    v = 1 << 20
+    c = (-0.69 * torch.rand(rows, generator=torch.Generator().manual_seed(rows))).to(dtype)
+    one = torch.ones(v)
+    if every:
+        one[every - 1::every] = -1
+    one[::509] = 0
+    others, zeros = int((one > 0).sum()), int((one == 0).sum())
+    one = one.to(dev)
+    z = torch.where(one == 1, c.to(dev)[:, None], (one.clamp(max=0) * torch.inf).nan_to_num(
+        0, neginf=-torch.inf).to(dtype))
+    c = c.double()
+    log_r = c + math.log(others)                               # of the others, below 0's
+    norm = torch.logaddexp(log_r, torch.full((), math.log(zeros)).double())
+    off = C.U * (6.1 + 80 + 2 * norm)
+    out = cb.profile_log_probs(z)
+    C.same(out.log_normalizer, norm, off, "normaliser")
+    # sum of x e over s, x = c or 0: each term is off by one rounding more, the quotient by two
+    share = torch.exp(log_r - norm)
+    h = norm - c * share
+    C.same(out.entropy, h, off + (6.1 + 80 + 6.1 + 80 + 4) * C.U * (c * share).abs()
+           + 2 * C.U * h, "entropy")
+    # half of the teacher's mass is the entry 0's: half of the normaliser's error reaches the loss
+    idx = torch.zeros(rows, 1, dtype=torch.int64, device=dev)
+    lp = torch.full((rows, 1), math.log(0.5), device=dev)
+    p = lp[0, 0].double().exp().item()
+    loss = cb.distillation_loss(z, idx, lp, reduction="none")
+    rest = torch.logaddexp(log_r, torch.full((), math.log(zeros - 1)).double())
+    want = p * (math.log(p) + norm) + (1 - p) * (math.log(1 - p) - (rest - norm))
+    C.same(loss, want, 0.5 * (6.1 + 80) * C.U + 4 * C.U * want, "loss")

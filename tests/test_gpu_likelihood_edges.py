@@ -41,3 +41,12 @@ def test_beside_forward_mode():
 
 def test_temperature_is_a_number():
     E.case_temperature_is_a_number(DEV)
+
+
+# a cluster to a row, and as many rows as give each one block
+@pytest.mark.parametrize("dtype,rows,every", [(F32, 3, 0), (F32, 900, 0), (F32, 3, 8),
+                                              (F32, 900, 8), (BF16, 900, 0), (BF16, 900, 8)])
+def test_long_sums(dtype, rows, every):
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB of free device memory")
+    E.case_long_sums(DEV, dtype, rows, every)

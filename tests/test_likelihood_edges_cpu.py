@@ -83,3 +83,8 @@ def test_exp64(tmp_path):
     assert off < 1e-14
     assert f(-700.1) == f(-math.inf) == 0.0 and f(700.1) == f(math.inf) == math.inf
     assert math.isnan(f(math.nan)) and f(0.0) == 1.0
+
+
+@pytest.mark.parametrize("every", [0, 8])
+def test_long_sums(every):
+    E.case_long_sums(DEV, F32, 2, every)
