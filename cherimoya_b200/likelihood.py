@@ -251,8 +251,9 @@ def _cpu_log_probs_backward(logits, mask, groups, targets, top_indices, stats, e
     if g_h is not None:
         d = d - torch.where(q > 0, q * (lq + entropy.reshape(R, 1)), 0.0) * g_h.reshape(R, 1)
     if idx.shape[1] and z.shape[1]:
-        d.scatter_add_(-1, idx.clamp(0, z.shape[1] - 1),
-                       torch.where((idx < 0) | past, 0.0, g))
+        at = torch.zeros(z.shape, dtype=torch.float64).scatter_add_(
+            -1, idx.clamp(0, z.shape[1] - 1), torch.where((idx < 0) | past, 0.0, g).double())
+        d = d + at.float()
     return _cpu_write(logits, torch.where(z == float("-inf"), 0.0, d / temperature), groups)
 
 

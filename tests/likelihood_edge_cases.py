@@ -179,3 +179,24 @@ def case_long_sums(dev, dtype, rows, every):
     rest = torch.logaddexp(log_r, torch.full((), math.log(zeros - 1)).double())
     want = p * (math.log(p) + norm) + (1 - p) * (math.log(1 - p) - (rest - norm))
     C.same(loss, want, 0.5 * (6.1 + 80) * C.U + 4 * C.U * want, "loss")
+
+
+def case_one_target(dev, v):
+    """1,024 targets that are one entry, with one gradient each that differs from row to row: the
+    roundings of their sum G have one sign. Terms are added at most 64 in a row, with 16 joins: 80 U
+    of G; the first term of the gradient, q G, is off by 2 CHAIN U of itself, as in
+    likelihood_common.py."""
+    rows = 64
+    z, g = C.logits((rows, v), torch.float32, v)
+    t = torch.full((rows, 1024), v // 3, dtype=torch.int64)
+    each = 0.5 + torch.rand(rows, 1, generator=g)
+    z = z.to(dev).requires_grad_()
+    out = cb.profile_log_probs(z, t.to(dev))
+    grad, = torch.autograd.grad(out.log_probs, z, each.expand(rows, 1024).to(dev))
+    total = 1024 * each.double()
+    q = torch.softmax(z.detach().double().cpu(), -1)
+    want = -q * total
+    tol = 2 * C.CHAIN * C.U * want.abs()
+    want[:, v // 3] += total[:, 0]
+    tol[:, v // 3] += 80 * C.U * total[:, 0]
+    C.same(grad, want, tol + 2 * C.U * want.abs() + C.TINY[torch.float32], "gradient")

@@ -50,3 +50,8 @@ def test_long_sums(dtype, rows, every):
     if torch.cuda.mem_get_info()[0] < 12 << 30:
         pytest.skip("needs 12 GB of free device memory")
     E.case_long_sums(DEV, dtype, rows, every)
+
+
+@pytest.mark.parametrize("v", [900, 40000])
+def test_one_target(v):
+    E.case_one_target(DEV, v)

@@ -88,3 +88,8 @@ def test_exp64(tmp_path):
 @pytest.mark.parametrize("every", [0, 8])
 def test_long_sums(every):
     E.case_long_sums(DEV, F32, 2, every)
+
+
+@pytest.mark.parametrize("v", [900, 40000])
+def test_one_target(v):
+    E.case_one_target(DEV, v)
