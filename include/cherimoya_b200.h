@@ -224,9 +224,10 @@ typedef struct {
  * the row gives NaN, one that does not take part -inf), the entropy, the log
  * normaliser, and the top_k most likely entries in descending order, equal
  * logits by ascending index (places without an entry: -inf and index -1).
- * Outputs fp32 (indices int64); each may be NULL when it is not wanted. stats
- * (rows, 2) keeps the row's maximum and its sum of exp((z - maximum) / T),
- * which the backward call reads. */
+ * Outputs fp32 (indices int64). entropy, log_normalizer and stats may be NULL
+ * when they are not wanted; log_probs may be with n_targets 0, and the two top
+ * arrays may be with top_k 0. stats (rows, 2) keeps the row's maximum and its
+ * sum of exp((z - maximum) / T), which the backward call reads. */
 int32_t chm_log_probs(const chm_rows* rows, const int64_t* targets, int32_t n_targets,
                       int32_t top_k, float* log_probs, float* entropy, float* log_normalizer,
                       float* top_log_probs, int64_t* top_indices, float* stats,

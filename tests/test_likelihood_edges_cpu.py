@@ -93,3 +93,15 @@ def test_long_sums(every):
 @pytest.mark.parametrize("v", [900, 40000])
 def test_one_target(v):
     E.case_one_target(DEV, v)
+
+
+def test_abi_outputs_that_may_not_be_null():
+    """Of chm_log_probs' outputs those of given and top entries are needed where there are such."""
+    lib = _lib.load()
+    off, size = (ctypes.c_int64 * 1)(0), (ctypes.c_int32 * 1)(10)
+    bogus = 64                                   # aligned, never dereferenced
+    rows = _lib.Rows(bogus, 0, 1, 2, 10, ctypes.addressof(off), ctypes.addressof(size), None, 0,
+                     None, None, 0, None, 1.0)
+    for s, k, lp, top, at in ((1, 0, None, None, None), (1, 1, None, bogus, bogus),
+                              (0, 1, None, None, bogus), (0, 1, None, bogus, None)):
+        assert lib.chm_log_probs(rows, bogus, s, k, lp, None, None, top, at, None, None) == 1
