@@ -200,3 +200,50 @@ def case_one_target(dev, v):
     want[:, v // 3] += total[:, 0]
     tol[:, v // 3] += 80 * C.U * total[:, 0]
     C.same(grad, want, tol + 2 * C.U * want.abs() + C.TINY[torch.float32], "gradient")
+
+
+def case_compiled(dev, dynamic):
+    """The public calls in compiled functions, without a graph break: the results of the plain
+    calls, bit for bit, forward and backward."""
+    g = torch.Generator().manual_seed(12)
+    groups = [1, 2]
+    t = torch.randint(0, 90, (4, 2, 5), generator=g)
+    t[0] = -1
+    idx = torch.stack([torch.randperm(90, generator=g)[:6] for _ in range(8)]).reshape(4, 2, 6)
+    lp = torch.log_softmax(torch.randn(4, 2, 6, generator=g), -1) - 0.1
+    w = 0.5 + torch.rand(4, 2, generator=g)
+    mask = (torch.rand(4, 3, 90, generator=g) < 0.9).to(dev)
+    t, idx, lp, w = t.to(dev), idx.to(dev), lp.to(dev), w.to(dev)
+    how = dict(signal_groups=groups, temperature=1.5, mask=mask)
+
+    def scores(z):
+        out = cb.profile_log_probs(z, t, top_k=3, **how)
+        return out.log_probs, out.entropy, out.log_normalizer, out.top_log_probs, out.top_indices
+
+    def losses(z):
+        return (cb.distillation_loss(z, idx, lp, weight=w, **how),
+                cb.distillation_loss(z, idx, lp, reduction="none", renormalize=True, **how))
+
+    def once(z):
+        return cb.distillation_loss_and_grad(z, idx, lp, weight=w, **how)
+
+    torch._dynamo.reset()
+    for f, with_grad in ((scores, 4), (losses, 2), (once, 0)):
+        compiled = torch.compile(f, backend="aot_eager", fullgraph=True, dynamic=dynamic)
+        for seed in (1, 2):
+            z = torch.randn(4, 3, 90, generator=torch.Generator().manual_seed(seed)).to(dev)
+            with torch.no_grad():
+                assert all(torch.equal(a, b) for a, b in zip(compiled(z), f(z)))
+            grads = []
+            for call in (f, compiled):
+                x = z.clone().requires_grad_()
+                out = call(x)
+                if with_grad:
+                    torch.manual_seed(seed)
+                    up = [torch.randn(o.shape).to(dev) for o in out[:with_grad]]
+                    grads.append(torch.autograd.grad(out[:with_grad], x, up)[0])
+                else:
+                    assert not any(o.requires_grad for o in out)
+                    grads.append(out[1])
+            assert torch.equal(*grads)
+    torch._dynamo.reset()

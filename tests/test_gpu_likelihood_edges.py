@@ -55,3 +55,35 @@ def test_long_sums(dtype, rows, every):
 @pytest.mark.parametrize("v", [900, 40000])
 def test_one_target(v):
     E.case_one_target(DEV, v)
+
+
+@pytest.mark.filterwarnings("ignore:Dynamo detected a call to a .functools.lru_cache")
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_compiled(dynamic):
+    E.case_compiled(DEV, dynamic)
+
+
+def test_custom_ops_check():
+    """The three custom ops behind compiled calls: their schemas, fake implementations and
+    dispatch, as torch.library checks them."""
+    from cherimoya_b200 import ops
+    tests = ("test_schema", "test_faketensor", "test_aot_dispatch_dynamic")
+    g = torch.Generator().manual_seed(3)
+    z = torch.randn(4, 3, 50, generator=g).to(DEV)
+    t = torch.randint(0, 50, (4, 2, 5), generator=g).to(DEV)
+    lp = torch.full((4, 2, 5), -2.0, device=DEV)
+    m = torch.rand(4, 3, 50, generator=g).to(DEV) < 0.8
+    w, up = torch.rand(4, 2, generator=g).to(DEV), torch.randn((), generator=g).to(DEV)
+    for mask in (None, m):
+        for stats in (False, True):
+            torch.library.opcheck(ops.log_probs, (z, mask, [1, 2], t, 3, 1.5, stats),
+                                  test_utils=tests)
+        out = ops.log_probs(z, mask, [1, 2], t, 3, 1.5, True)
+        torch.library.opcheck(ops.log_probs_backward,
+                              (z, mask, [1, 2], t, out[4], out[5], out[1], lp, w, None, None, 1.5),
+                              test_utils=tests)
+        for weight, upstream, reduce, grad in ((None, None, False, True), (w, up, True, True),
+                                               (w, w, False, True), (None, None, True, False)):
+            torch.library.opcheck(ops.distill, (z, mask, [1, 2], t, lp, False, weight, 0.25,
+                                                upstream, not reduce, reduce, grad, 1.5),
+                                  test_utils=tests)

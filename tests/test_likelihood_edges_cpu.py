@@ -105,3 +105,9 @@ def test_abi_outputs_that_may_not_be_null():
     for s, k, lp, top, at in ((1, 0, None, None, None), (1, 1, None, bogus, bogus),
                               (0, 1, None, None, bogus), (0, 1, None, bogus, None)):
         assert lib.chm_log_probs(rows, bogus, s, k, lp, None, None, top, at, None, None) == 1
+
+
+@pytest.mark.filterwarnings("ignore:Dynamo detected a call to a .functools.lru_cache")
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_compiled(dynamic):
+    E.case_compiled(DEV, dynamic)
