@@ -505,7 +505,7 @@ __device__ __noinline__ Sums careful_sums(const Row<T>& row, const Share<T>& sha
     uint4 r[1] = {*reinterpret_cast<const uint4*>(row.vec(j))};
     if (kMask) row.apply_mask(r[0], j);
     accumulate<T, 1, true, true>(r, Vec<T>::max(r[0]), c, part);
-    if (++n % 16 == 0) {                          // few roundings in a row
+    if (++n % kMaxBatches == 0) {
       sum = join(sum, part, c);
       part = {neg_inf(), 0.f, 0.f};
     }
