@@ -1202,13 +1202,15 @@ log_probs_grad_kernel(const __grid_constant__ Rows a, const ScoreGradArgs o, uns
   for (int k = Tm::tid(); k < n; k += kThreads) {
     const int v = key_entry(key[k]);
     if (v < share.first || v >= share.last || (k > 0 && key_entry(key[k - 1]) == v)) continue;
-    float at = 0.f;
-    for (int q = k; q < n && key_entry(key[q]) == v;) {
-      float part = 0.f;                           // few roundings in a row
-      for (const int end = min(q + 32, n); q < end && key_entry(key[q]) == v; ++q)
-        part += g[key_place(key[q])];
-      at += part;
+    float at = 0.f, part = g[key_place(key[k])];
+    for (int q = k + 1; q < n && key_entry(key[q]) == v; ++q) {
+      if ((q - k) % 32 == 0) {                    // few roundings in a row
+        at += part;
+        part = 0.f;
+      }
+      part += g[key_place(key[q])];
     }
+    at += part;
     put(v, at);
   }
 }
