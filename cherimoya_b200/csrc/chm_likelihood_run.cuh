@@ -49,9 +49,10 @@ Cut cut_rows(int nvec, long long rows, bool warp) {
 // takes up to 16 vectors a lane: 2,048 examples of five groups of 1,000 and 2,000
 // masked fp32 entries take 50 us, 56 with teams of 64 and 79 with 128. Longer rows get
 // a block of 128 (4,096 x 50,001 bf16: 88 us, 109 with 256), more than 64 top
-// entries too, since a lane keeps at most two; few long rows are shared by the
-// blocks of a cluster, and so are rows of which a thread would add up more than
-// kMaxBatches batches one by one.
+// entries too: near as many as a warp's 128 maxima, they are bounded so loosely that most of the
+// row is a candidate (10,240 x 1,000 with 128 of them 156 us, a warp per row 381; with 65
+// it is 84 and 52). Few long rows are shared by the blocks of a cluster, and so are rows of which
+// a thread would add up more than kMaxBatches batches one by one.
 Cut cut_stream(int nvec, long long rows, int top_k) {
   Cut c{};
   c.threads = nvec <= 512 && top_k <= 64 ? 32 : 128;
@@ -166,8 +167,9 @@ int run_distill_m(const Rows& a, const DistillArgs& o, long long n, cudaStream_t
     // chunks of 8 KB, the next on its way while it sums one, and seven blocks fit
     // an SM: 1,024 x 100,003 fp32 entries take 85 us (16 KB: 95; 32 KB and 256
     // threads: 96), 2,048 x 100,003 bf16 93 (103; 118), 4,096 x 25,000 fp32 83
-    // (84; 104), 8,192 x 12,000 bf16 79 (held whole: 120). Below 16 KB a row is
-    // one chunk. Few rows are cut until there are three blocks to an SM.
+    // (84; 104), 8,192 x 12,000 bf16 79 (held whole: 120); 500 x 100,003 fp32 lose (54 to 57,
+    // 50 with 16 KB). Below 16 KB a row is one chunk. Few rows are cut until there are three
+    // blocks to an SM; up to seven gave 500 x 100,003 50 but 250 x 100,003 38 instead of 35.
     c = {128, 0, 512};
     while (c.log_blocks < 3 && n << c.log_blocks < 3 * 148 && nvec >> c.log_blocks > 2048)
       ++c.log_blocks;

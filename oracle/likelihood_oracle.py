@@ -25,15 +25,6 @@ def split_rows(x, groups):
     return rows
 
 
-def join_rows(rows, shape, groups):
-    if groups is None:
-        return torch.stack(rows).reshape(shape)
-    per = len(groups)
-    return torch.stack([torch.cat([r.reshape(g, shape[2]) for r, g in
-                                   zip(rows[i:i + per], groups)]) for i in
-                        range(0, len(rows), per)]).reshape(shape)
-
-
 def _row(z, mask, T):
     z = z.double().clone()
     if mask is not None:
