@@ -7,6 +7,7 @@ import torch
 
 import cherimoya_b200 as cb
 import likelihood_common as C
+from oracle import likelihood_oracle as LO
 
 
 def case_candidates(dev, dtype, v, rows):
@@ -247,3 +248,34 @@ def case_compiled(dev, dynamic):
                     grads.append(out[1])
             assert torch.equal(*grads)
     torch._dynamo.reset()
+
+
+def case_many_long_rows(dev, dtype, masked, copies):
+    """Long rows, many of them, so that each has a block: three rows, each there `copies` times,
+    with 600 listed entries, some of them twice, at both ends and not part of the mask."""
+    v, k = 300001 if dtype == torch.float32 else 600001, 600
+    z, g = C.logits((3, v), dtype, 77)
+    idx = torch.randint(0, v, (3, k), generator=g)
+    idx[:, :4] = torch.tensor([0, v - 1, 3, v - 2])
+    idx[:, 4:8] = idx[:, 8:12]
+    lp = torch.log_softmax(torch.randn(3, k, generator=g), -1) - 0.4
+    mask = torch.rand(3, v, generator=g) < 0.8 if masked else None
+    want, mags, off = [], [], []
+    for r in range(3):
+        m = mask[r] if masked else None
+        loss, mag, _, _ = LO.distill_row(z[r], m, idx[r], lp[r], False, 1.0)
+        want.append(loss)
+        mags.append(2 * C.CHAIN * C.U * (mag + 1))
+        s = LO.score_row(z[r], m, idx[r, :0], 0, 1.0)
+        off.append((s["log_normalizer"], C.U * (4 * abs(s["log_s"]) + C.CHAIN)
+                    + 4 * C.U * abs(s["log_normalizer"])))
+    many = lambda t: t.to(dev).repeat(copies, *[1] * (t.dim() - 1))
+    zl, ml = many(z), many(mask) if masked else None
+    loss = cb.distillation_loss(zl, many(idx), many(lp), mask=ml, reduction="none")
+    C.same(loss, torch.tensor(want * copies), torch.tensor(mags * copies), "losses")
+    out = cb.profile_log_probs(zl, mask=ml, top_k=5)
+    norm, tol = torch.tensor(off).double().unbind(-1)
+    C.same(out.log_normalizer, norm.repeat(copies), tol.repeat(copies), "normaliser")
+    seen = torch.where(mask, z, -torch.inf) if masked else z
+    at = torch.sort(seen.float(), dim=-1, descending=True, stable=True)[1][:, :5]
+    assert torch.equal(out.top_indices.cpu(), at.repeat(copies, 1))

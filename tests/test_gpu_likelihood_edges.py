@@ -87,3 +87,9 @@ def test_custom_ops_check():
             torch.library.opcheck(ops.distill, (z, mask, [1, 2], t, lp, False, weight, 0.25,
                                                 upstream, not reduce, reduce, grad, 1.5),
                                   test_utils=tests)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_many_long_rows(dtype, masked):
+    E.case_many_long_rows(DEV, dtype, masked, 150)

@@ -111,3 +111,8 @@ def test_abi_outputs_that_may_not_be_null():
 @pytest.mark.parametrize("dynamic", [False, True])
 def test_compiled(dynamic):
     E.case_compiled(DEV, dynamic)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_long_rows(masked):
+    E.case_many_long_rows(DEV, F32, masked, 1)
